@@ -1,0 +1,87 @@
+// k3_rowops.h -- device helpers shared by the operators that work on rows of float / half / bfloat16 matrices (k3_layernorm.hip, k3_objf.hip) and by k3_affine.hip.
+#pragma once
+#include "k3_common.h"
+
+namespace k3 {
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+
+// 16 bytes of a row.  The alignment is the element's: rows may start anywhere (odd widths, padded strides), and gfx950's global loads and stores of four registers take any address.
+template <typename T> struct Chunk { static constexpr int N = 16 / (int)sizeof(T); typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T)))); };
+
+template <typename T> __device__ inline float to_f32(T v) { return (float)v; }
+
+// lanes of a wavefront: inclusive combination over DPP row shifts and the two row broadcasts, complete in lane 63, in a fixed order
+template <int CTRL, int ROW_MASK> __device__ inline float dpp_f32(float identity, float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, identity), __builtin_bit_cast(int, v), CTRL, ROW_MASK, 0xf, false));
+}
+__device__ inline float lane63(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63)); }
+__device__ inline float wave_sum(float v) {
+  v += dpp_f32<0x111, 0xf>(0.0f, v);      // row_shr 1, 2, 4, 8
+  v += dpp_f32<0x112, 0xf>(0.0f, v);
+  v += dpp_f32<0x114, 0xf>(0.0f, v);
+  v += dpp_f32<0x118, 0xf>(0.0f, v);
+  v += dpp_f32<0x142, 0xa>(0.0f, v);      // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+  v += dpp_f32<0x143, 0xc>(0.0f, v);
+  return lane63(v);
+}
+__device__ inline float wave_max(float v) {      // NaNs are passed over (as fmaxf does)
+  const float id = -__builtin_inff();
+  v = fmaxf(v, dpp_f32<0x111, 0xf>(id, v));
+  v = fmaxf(v, dpp_f32<0x112, 0xf>(id, v));
+  v = fmaxf(v, dpp_f32<0x114, 0xf>(id, v));
+  v = fmaxf(v, dpp_f32<0x118, 0xf>(id, v));
+  v = fmaxf(v, dpp_f32<0x142, 0xa>(id, v));
+  v = fmaxf(v, dpp_f32<0x143, 0xc>(id, v));
+  return lane63(v);
+}
+
+// the same over NW wavefronts of a workgroup; `sh` holds NW values per call and is free again after the NEXT barrier: consecutive calls take different buffers
+template <int NW> __device__ inline float block_sum(float v, float *sh) {
+  v = wave_sum(v);
+  if constexpr (NW > 1) {
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) v += sh[w];
+  }
+  return v;
+}
+template <int NW> __device__ inline float block_max(float v, float *sh) {
+  v = wave_max(v);
+  if constexpr (NW > 1) {
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < NW; w++) v = fmaxf(v, sh[w]);
+  }
+  return v;
+}
+// two sums at once (sh: 2 NW values)
+template <int NW> __device__ inline void block_sum2(float &a, float &b, float *sh) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if constexpr (NW > 1) {
+    if ((threadIdx.x & 63) == 0) { sh[2 * (threadIdx.x >> 6)] = a; sh[2 * (threadIdx.x >> 6) + 1] = b; }
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) { a += sh[2 * w]; b += sh[2 * w + 1]; }
+  }
+}
+
+inline bool dtype_ok(int dtype) { return dtype >= K3_F32 && dtype <= K3_BF16; }
+inline size_t dtype_size(int dtype) { return dtype == K3_F32 ? 4 : 2; }
+
+}  // namespace k3
+
+// f(T{}) for the type of a k3_dtype that has been checked
+#define K3_FOR_DTYPE(dtype, f)                                     \
+  do {                                                             \
+    if ((dtype) == K3_F32) { f(float); }                           \
+    else if ((dtype) == K3_F16) { f(k3::f16); }                    \
+    else { f(k3::bf16); }                                          \
+  } while (0)

@@ -6,6 +6,38 @@ from . import lib as _l
 
 def _st(): return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
+# ---- arguments of the operators that take matrices of any k3_dtype: CuMatrix objects or 2-dimensional tensors whose rows are contiguous, all on one device (which need not be
+# the current one); the kernels run on that device's current stream
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # k3_dtype
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
+
+def _refuse(what): raise _l.K3Error(what)
+def _rows(m, name):
+    """the tensor behind a matrix argument, checked, and its leading dimension"""
+    t = m.t if isinstance(m, CuMatrix) else m
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype not in _DTYPES: _refuse(f"{name}: a matrix of float32, float16 or bfloat16 is wanted")
+    if not t.is_cuda: _refuse(f"{name}: not on a GPU")
+    r, c = t.shape
+    s0, s1 = t.stride()
+    if (c > 1 and s1 != 1) or (r > 1 and s0 < c): _refuse(f"{name}: rows must be contiguous and must not overlap (strides {s0}, {s1})")
+    return t, (s0 if r > 1 else c)
+def _like_rows(m, ref, name, dtype=True):
+    """a second matrix of ref's shape, device and (unless dtype is False) type"""
+    t, ld = _rows(m, name)
+    if t.shape != ref.shape or t.device != ref.device or (dtype and t.dtype != ref.dtype): _refuse(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device} does not go with {tuple(ref.shape)} {ref.dtype} on {ref.device}")
+    return t, ld
+def _vec(t, shape, ref, name, dtype=torch.float32):
+    """pointer of a contiguous tensor of that shape (None: null)"""
+    if t is None: return None
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.device != ref.device: _refuse(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {ref.device} is wanted")
+    return t.data_ptr()
+def _run(ref, f, *args):
+    """f(*args, stream) on ref's device"""
+    i = ref.device.index
+    if i == torch.cuda.current_device(): _l.check(f(*args, _raw_stream(i)))
+    else:
+        with torch.cuda.device(i): _l.check(f(*args, _raw_stream(i)))
+
 class CuMatrix:
     def __init__(self, t):
         assert t.is_cuda and t.dtype == torch.float32 and t.dim() == 2 and t.stride(1) == 1
@@ -78,6 +110,25 @@ def NormalizePerRow(inp, target_rms, add_log_stddev, out):      # cu::NormalizeP
 def DiffNormalizePerRow(in_value, out_deriv, target_rms, add_log_stddev, in_deriv):      # cu::DiffNormalizePerRow (cudamatrix/cu-math.h:296): ADDS to in_deriv unless it is out_deriv
     assert out_deriv.NumCols() == in_value.NumCols() + int(add_log_stddev) and in_deriv.NumCols() == in_value.NumCols()
     _l.check(in_deriv._L.k3_mat_normalize_rows(1, in_deriv.t.data_ptr(), in_deriv.Stride(), in_value.t.data_ptr(), in_value.Stride(), out_deriv.t.data_ptr(), out_deriv.Stride(), in_value.NumRows(), in_value.NumCols(), target_rms, int(add_log_stddev), _st()))
+
+def LayerNormPerRow(inp, scale, offset, eps, out, mean=None, inv_std=None):
+    """Layer norm: out = (inp - mean) inv_std scale + offset row by row, inv_std = 1 / sqrt(var + eps).  inp, out: matrices of one type (float32, float16, bfloat16), out may be inp;
+    scale, offset: float32 vectors of the row length or None; mean, inv_std: float32 vectors of the number of rows that receive the statistics DiffLayerNormPerRow takes, or None."""
+    x, ldx = _rows(inp, "inp"); y, ldy = _like_rows(out, x, "out"); r, c = x.shape
+    if not 0.0 <= eps < float("inf"): _refuse(f"eps: {eps}")
+    _run(x, _l.load().k3_layer_norm_forward, _DTYPES[x.dtype], x.data_ptr(), ldx, _vec(scale, (c,), x, "scale"), _vec(offset, (c,), x, "offset"), eps, y.data_ptr(), ldy,
+         _vec(mean, (r,), x, "mean"), _vec(inv_std, (r,), x, "inv_std"), r, c)
+def DiffLayerNormPerRow(in_value, out_deriv, scale, mean, inv_std, in_deriv=None, scale_deriv=None, offset_deriv=None, accumulate=False):
+    """The backward pass of LayerNormPerRow from its input, its kept statistics and the derivative with respect to its output.  in_deriv (may be out_deriv or in_value) is overwritten;
+    scale_deriv, offset_deriv (float32 vectors) are overwritten, or added to with accumulate.  What is None is not computed."""
+    x, ldx = _rows(in_value, "in_value"); g, ldg = _like_rows(out_deriv, x, "out_deriv"); r, c = x.shape
+    if mean is None or inv_std is None: _refuse("mean, inv_std: the statistics of the forward pass are wanted")
+    d, ldd = (None, c) if in_deriv is None else _like_rows(in_deriv, x, "in_deriv")
+    L = _l.load(); ws = None
+    if scale_deriv is not None or offset_deriv is not None: ws = torch.empty(L.k3_layer_norm_backward_workspace(r, c), dtype=torch.uint8, device=x.device)
+    _run(x, L.k3_layer_norm_backward, _DTYPES[x.dtype], x.data_ptr(), ldx, g.data_ptr(), ldg, _vec(scale, (c,), x, "scale"), _vec(mean, (r,), x, "mean"), _vec(inv_std, (r,), x, "inv_std"),
+         None if d is None else d.data_ptr(), ldd, _vec(scale_deriv, (c,), x, "scale_deriv"), _vec(offset_deriv, (c,), x, "offset_deriv"), int(accumulate),
+         None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), r, c)
 
 class CuRand:
     """CuRand<BaseFloat> (cudamatrix/cu-rand.h:31-64) over k3_mat_set_rand: one seed per object, the counter position advances by what each fill consumes"""

@@ -157,6 +157,9 @@ def load():
     L.k3_mat_copy_cols.argtypes = [i32, vp, i64, i32, i32, vp, i64, vp, vp]
     L.k3_mat_add_diag_vec_mat.argtypes = [f32, vp, vp, i64, i32, f32, vp, i64, i32, i32, vp]; L.k3_mat_div_elements.argtypes = [vp, i64, i32, i32, vp, i64, vp]; L.k3_mat_reduce_scalar.argtypes = [i32, vp, i64, vp, i64, i32, i32, vp, vp]
     L.k3_vec_col_reduce.argtypes = [i32, f32, vp, i64, vp, i64, i32, i32, f32, vp, vp]
+    L.k3_layer_norm_forward.argtypes = [i32, vp, i64, vp, vp, f32, vp, i64, vp, vp, i32, i32, vp]
+    L.k3_layer_norm_backward_workspace.argtypes = [i32, i32]; L.k3_layer_norm_backward_workspace.restype = i64
+    L.k3_layer_norm_backward.argtypes = [i32, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, i32, vp, i64, i32, i32, vp]
     L.k3_chain_den_create.argtypes = [i32, i32, i32, vp, vp, vp, vp, vp, ctypes.POINTER(vp)]; L.k3_chain_den_destroy.argtypes = [vp]; L.k3_chain_den_destroy.restype = None
     L.k3_chain_den_num_states.argtypes = [vp]; L.k3_chain_den_initial_probs.argtypes = [vp, vp]
     L.k3_chain_den_forward_backward.argtypes = [vp, vp, i64, i32, i32, f32, f32, vp, i64, ctypes.POINTER(f32), ctypes.POINTER(i32), vp]
