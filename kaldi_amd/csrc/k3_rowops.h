@@ -12,6 +12,35 @@ template <typename T> struct Chunk { static constexpr int N = 16 / (int)sizeof(T
 
 template <typename T> __device__ inline float to_f32(T v) { return (float)v; }
 
+// chunk i of a row: `valid` elements of it exist (the rest is zero).  Rows end inside a chunk, never across one that is read past its end
+template <typename T> __device__ inline typename Chunk<T>::type load_chunk(const T *row, int col, int valid) {
+  typename Chunk<T>::type v;
+  if (valid >= Chunk<T>::N) return *reinterpret_cast<const typename Chunk<T>::type *>(row + col);
+#pragma unroll
+  for (int j = 0; j < Chunk<T>::N; j++) v[j] = j < valid ? row[col + j] : (T)0.0f;
+  return v;
+}
+template <typename T> __device__ inline void store_chunk(T *row, int col, int valid, typename Chunk<T>::type v) {
+  if (valid >= Chunk<T>::N) { *reinterpret_cast<typename Chunk<T>::type *>(row + col) = v; return; }
+#pragma unroll
+  for (int j = 0; j < Chunk<T>::N; j++) if (j < valid) row[col + j] = v[j];
+}
+// N floats from a vector (null: `otherwise`)
+template <int N> __device__ inline void load_params(const float *p, int col, int valid, float otherwise, float *out) {
+  typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+  if (p && valid >= N) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+      const f4 v = *reinterpret_cast<const f4 *>(p + col + j);
+#pragma unroll
+      for (int k = 0; k < 4; k++) out[j + k] = v[k];
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < N; j++) out[j] = p && j < valid ? p[col + j] : otherwise;
+}
+
 // lanes of a wavefront: inclusive combination over DPP row shifts and the two row broadcasts, complete in lane 63, in a fixed order
 template <int CTRL, int ROW_MASK> __device__ inline float dpp_f32(float identity, float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, identity), __builtin_bit_cast(int, v), CTRL, ROW_MASK, 0xf, false));
