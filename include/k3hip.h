@@ -576,6 +576,30 @@ int64_t k3_layer_norm_backward_workspace(int32_t rows, int32_t cols);
 int k3_layer_norm_backward(int32_t dtype, const void *d_x, int64_t ldx, const void *d_dy, int64_t lddy, const float *d_scale, const float *d_mean, const float *d_inv_std,
                            void *d_dx, int64_t lddx, float *d_dscale, float *d_doffset, int32_t accumulate, void *d_workspace, int64_t workspace_bytes,
                            int32_t rows, int32_t cols, void *stream);
+/* Scores of the rows of a network's output z: the log-probability log q_y of one label y per row under the row's softmax, the row's entropy -sum q log q, and its num_alternatives
+ * (0 .. 64) most probable columns with their log-probabilities, best first, equal ones by column.  Stands beside CuMatrixBase::LogSoftMaxPerRow (cudamatrix/cu-matrix.h:334), without
+ * the matrix of log-probabilities.  d_labels [rows] (a label outside 0 .. cols - 1, -1 for instance, = none: its log-probability is 0); every output may be null: d_log_prob, d_entropy
+ * [rows]; d_stats [rows][2] = the row's largest value and ln sum exp(z - it), which the derivative takes; d_alt_log_probs, d_alt_labels [rows][num_alternatives].
+ * -inf in z = a column that cannot be (probability 0).  A row of nothing but -inf has log-probabilities -inf and entropy 0; one that holds a NaN or +inf has NaN scores and no
+ * alternatives (-1).  At most 2^21 columns.  Workspace (16-byte aligned, may be null where 0 bytes are asked for): k3_label_logprobs_workspace. */
+int64_t k3_label_logprobs_workspace(int32_t dtype, int32_t rows, int32_t cols, int32_t num_alternatives);
+int k3_label_logprobs(int32_t dtype, const void *d_z, int64_t ld, const int32_t *d_labels, float *d_log_prob, float *d_entropy, float *d_stats, int32_t num_alternatives,
+                      float *d_alt_log_probs, int32_t *d_alt_labels, void *d_workspace, int64_t workspace_bytes, int32_t rows, int32_t cols, void *stream);
+/* The derivative of sum_r d_log_prob_deriv[r] log q_y(r) + d_entropy_deriv[r] entropy(r) with respect to z, into d_dz (overwritten; may be z).  d_stats (and d_entropy, where
+ * d_entropy_deriv is given) are the forward pass's; either derivative may be null (0); a row without a label has no first term; a row of nothing but -inf gets zeros. */
+int k3_label_logprobs_deriv(int32_t dtype, const void *d_z, int64_t ld, const int32_t *d_labels, const float *d_stats, const float *d_entropy, const float *d_log_prob_deriv,
+                            const float *d_entropy_deriv, void *d_dz, int64_t ldd, int32_t rows, int32_t cols, void *stream);
+/* Distillation from a teacher's top logits: row r has num_entries (1 .. 1024) pairs of a teacher value (of z's type) and its column; a column outside 0 .. cols - 1, -1 for instance =
+ * not used.  With p = softmax(values / T) over the used entries, q = softmax(z / T) over all columns and T = temperature:
+ *   d_objf[r] = w_r T^2 sum_k p_k (log q_{i_k} - log p_k)      (the negative divergence of p from q: to be maximised, as the chain objective is)
+ *   d_dz[r][j] = w_r T (sum of p_k over i_k = j  -  q_j)       (its derivative; overwritten, may be z; d_dz null: not wanted)
+ * A column may come more than once.  d_weights [rows] (null: 1).  A row without a used entry (or with nothing but -inf in them), or of weight 0, has objective 0 and zeros, whatever z
+ * holds; otherwise a row of z with nothing but -inf has objective -inf w_r and zeros.  One entry per row is the cross entropy.  At most 2^21 columns.
+ * Workspace (16-byte aligned, may be null where 0 bytes are asked for): k3_distill_workspace. */
+int64_t k3_distill_workspace(int32_t dtype, int32_t rows, int32_t cols, int32_t num_entries, int32_t with_deriv);
+int k3_distill_objf_and_deriv(int32_t dtype, float temperature, const void *d_z, int64_t ld, const void *d_teacher_values, int64_t ld_values, const int32_t *d_teacher_indexes,
+                              int64_t ld_indexes, int32_t num_entries, const float *d_weights, float *d_objf, void *d_dz, int64_t ldd, void *d_workspace,
+                              int64_t workspace_bytes, int32_t rows, int32_t cols, void *stream);
 
 #ifdef __cplusplus
 }

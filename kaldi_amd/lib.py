@@ -160,6 +160,11 @@ def load():
     L.k3_layer_norm_forward.argtypes = [i32, vp, i64, vp, vp, f32, vp, i64, vp, vp, i32, i32, vp]
     L.k3_layer_norm_backward_workspace.argtypes = [i32, i32]; L.k3_layer_norm_backward_workspace.restype = i64
     L.k3_layer_norm_backward.argtypes = [i32, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, i32, vp, i64, i32, i32, vp]
+    L.k3_label_logprobs_workspace.argtypes = [i32, i32, i32, i32]; L.k3_label_logprobs_workspace.restype = i64
+    L.k3_label_logprobs.argtypes = [i32, vp, i64, vp, vp, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp]
+    L.k3_label_logprobs_deriv.argtypes = [i32, vp, i64, vp, vp, vp, vp, vp, vp, i64, i32, i32, vp]
+    L.k3_distill_workspace.argtypes = [i32, i32, i32, i32, i32]; L.k3_distill_workspace.restype = i64
+    L.k3_distill_objf_and_deriv.argtypes = [i32, f32, vp, i64, vp, i64, vp, i64, i32, vp, vp, vp, i64, vp, i64, i32, i32, vp]
     L.k3_chain_den_create.argtypes = [i32, i32, i32, vp, vp, vp, vp, vp, ctypes.POINTER(vp)]; L.k3_chain_den_destroy.argtypes = [vp]; L.k3_chain_den_destroy.restype = None
     L.k3_chain_den_num_states.argtypes = [vp]; L.k3_chain_den_initial_probs.argtypes = [vp, vp]
     L.k3_chain_den_forward_backward.argtypes = [vp, vp, i64, i32, i32, f32, f32, vp, i64, ctypes.POINTER(f32), ctypes.POINTER(i32), vp]

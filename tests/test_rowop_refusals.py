@@ -21,8 +21,35 @@ def test_layer_norm_entry_points():
     refused(bwd(dtype=9), "type"); refused(bwd(ldx=7), "bad argument"); refused(bwd(ldg=7), "bad argument"); refused(bwd(ldd=7), "bad argument"); refused(bwd(mean=None), "null"); refused(bwd(x=None), "null")
     refused(bwd(ws=None), "workspace"); refused(bwd(n=need - 1), "workspace")
 
+def test_label_entry_points():
+    L = _l.load()
+    f = lambda dtype=0, z=P, ld=8, y=P, lp=P, n=0, al=None, ai=None, ws=None, nb=0, rows=4, cols=8: L.k3_label_logprobs(dtype, z, ld, y, lp, None, None, n, al, ai, ws, nb, rows, cols, None)  # noqa: E731
+    refused(f(dtype=3), "type"); refused(f(ld=7), "bad argument"); refused(f(rows=-1), "bad argument"); refused(f(cols=0), "bad argument"); refused(f(n=-1), "bad argument"); refused(f(z=None), "null"); refused(f(y=None), "null")
+    refused(f(n=65, al=P, cols=100, ld=100), "at most"); refused(f(cols=(1 << 21) + 1, ld=1 << 22), "at most"); refused(f(n=9, al=P), "more alternatives"); refused(f(n=3), "do not go together"); refused(f(al=P), "do not go together")
+    assert f(rows=0) == 0
+    need = L.k3_label_logprobs_workspace(0, 4, 100000, 5); assert need > 0 and L.k3_label_logprobs_workspace(0, 4000, 6024, 5) == 0
+    refused(f(cols=100000, ld=100000, n=5, al=P, ws=P, nb=need - 1), "workspace"); refused(f(cols=100000, ld=100000, n=5, al=P, ws=P + 4, nb=need), "workspace"); refused(f(cols=100000, ld=100000, n=5, al=P), "workspace")
+    g = lambda dtype=0, z=P, ld=8, y=P, st=P, h=P, a=P, b=P, dz=P, ldd=8, rows=4, cols=8: L.k3_label_logprobs_deriv(dtype, z, ld, y, st, h, a, b, dz, ldd, rows, cols, None)  # noqa: E731
+    refused(g(dtype=-1), "type"); refused(g(ld=7), "bad argument"); refused(g(ldd=7), "bad argument"); refused(g(cols=0), "bad argument"); refused(g(rows=-1), "bad argument")
+    for k in ("z", "st", "dz", "y", "h"): refused(g(**{k: None}), "null")
+    assert g(rows=0) == 0
+
+def test_distillation_entry_point():
+    L = _l.load()
+    f = lambda dtype=0, T=1.0, z=P, ld=8, v=P, ldv=3, i=P, ldi=3, n=3, o=P, dz=P, ldd=8, ws=None, nb=0, rows=4, cols=8: L.k3_distill_objf_and_deriv(dtype, T, z, ld, v, ldv, i, ldi, n, None, o, dz, ldd, ws, nb, rows, cols, None)  # noqa: E731
+    refused(f(dtype=3), "type")
+    for T in (0.0, -1.0, float("nan"), float("inf"), 1e-4): refused(f(T=T), "temperature")
+    for k in ("ld", "ldv", "ldi", "ldd"): refused(f(**{k: 2}), "bad argument")
+    refused(f(n=0), "bad argument"); refused(f(cols=0), "bad argument"); refused(f(rows=-1), "bad argument"); refused(f(n=1025, ldv=2000, ldi=2000), "at most"); refused(f(cols=(1 << 21) + 1, ld=1 << 22, ldd=1 << 22), "at most")
+    for k in ("z", "v", "i", "o"): refused(f(**{k: None}), "null")
+    assert f(rows=0) == 0
+    need = L.k3_distill_workspace(0, 4, 200000, 3, 1); assert need > 0 and L.k3_distill_workspace(0, 4, 6024, 3, 1) == 0
+    refused(f(cols=200000, ld=200000, ldd=200000, ws=P, nb=need - 1), "workspace"); refused(f(cols=200000, ld=200000, ldd=200000), "workspace"); refused(f(cols=200000, ld=200000, ldd=200000, ws=P + 8, nb=need), "workspace")
+
 def test_matrices_that_are_no_rows_on_a_gpu():
-    from kaldi_amd import cumatrix as cm
+    from kaldi_amd import cumatrix as cm, objective as ob
     t = torch.zeros(4, 8)
     for bad, word in ((t, "GPU"), (torch.zeros(4), "matrix"), (torch.zeros(4, 8, dtype=torch.float64), "matrix"), (torch.zeros(4, 8, dtype=torch.int32), "matrix"), ("x", "matrix")):
         with pytest.raises(K3Error, match=word): cm.LayerNormPerRow(bad, None, None, 1e-5, bad)
+        with pytest.raises(K3Error, match=word): ob.LabelLogProbs(bad, None)
+        with pytest.raises(K3Error, match=word): ob.ComputeDistillObjfAndDeriv(ob.DistillationOptions(), bad, bad, bad, None, None)
