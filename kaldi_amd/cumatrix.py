@@ -11,32 +11,45 @@ def _st(): return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # k3_dtype
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
 
+_current_device = torch.cuda.current_device
+_F32, _I32 = torch.float32, torch.int32
+_devices = [torch.device("cuda", i) for i in range(64)]
+
 def _refuse(what): raise _l.K3Error(what)
 def _rows(m, name):
-    """the tensor behind a matrix argument, checked, and its leading dimension"""
-    t = m.t if isinstance(m, CuMatrix) else m
-    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype not in _DTYPES: _refuse(f"{name}: a matrix of float32, float16 or bfloat16 is wanted")
-    if not t.is_cuda: _refuse(f"{name}: not on a GPU")
-    r, c = t.shape
-    s0, s1 = t.stride()
-    if (c > 1 and s1 != 1) or (r > 1 and s0 < c): _refuse(f"{name}: rows must be contiguous and must not overlap (strides {s0}, {s1})")
-    return t, (s0 if r > 1 else c)
-def _like_rows(m, ref, name, dtype=True):
-    """a second matrix of ref's shape, device and (unless dtype is False) type"""
-    t, ld = _rows(m, name)
-    if t.shape != ref.shape or t.device != ref.device or (dtype and t.dtype != ref.dtype): _refuse(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device} does not go with {tuple(ref.shape)} {ref.dtype} on {ref.device}")
-    return t, ld
-def _vec(t, shape, ref, name, dtype=torch.float32):
-    """pointer of a contiguous tensor of that shape (None: null)"""
+    """a matrix argument, checked: (k3_dtype, pointer, leading dimension, rows, columns, device index)"""
+    t = m.t if type(m) is CuMatrix else m
+    try: dt = _DTYPES[t.dtype]; r, c = t.shape; s0, s1 = t.stride(); i = t.get_device()
+    except (AttributeError, KeyError, ValueError, RuntimeError): _refuse(f"{name}: a matrix of float32, float16 or bfloat16 is wanted")
+    if i < 0: _refuse(f"{name}: not on a GPU")
+    if r <= 1: s0 = c
+    if (s1 != 1 and c > 1) or s0 < c: _refuse(f"{name}: rows must be contiguous and must not overlap (strides {s0}, {s1})")
+    return dt, t.data_ptr(), s0, r, c, i
+def _like_rows(m, x, name):
+    """a second matrix of x's shape, type and device (x: what _rows gave): (pointer, leading dimension)"""
+    y = _rows(m, name)
+    if y[3] != x[3] or y[4] != x[4] or y[0] != x[0] or y[5] != x[5]: _refuse(f"{name}: {y[3]} x {y[4]} of type {y[0]} on device {y[5]} does not go with {x[3]} x {x[4]} of type {x[0]} on device {x[5]}")
+    return y[1], y[2]
+def _vec(t, n, i, name, dtype=_F32):
+    """pointer of a contiguous vector of n elements on device i (None: null)"""
     if t is None: return None
-    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.device != ref.device: _refuse(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {ref.device} is wanted")
-    return t.data_ptr()
-def _run(ref, f, *args):
-    """f(*args, stream) on ref's device"""
-    i = ref.device.index
-    if i == torch.cuda.current_device(): _l.check(f(*args, _raw_stream(i)))
+    try:
+        if t.dtype is dtype and t.numel() == n and t.get_device() == i and t.is_contiguous(): return t.data_ptr()
+    except AttributeError: pass
+    _refuse(f"{name}: a contiguous {dtype} tensor of {n} elements on device {i} is wanted")
+def _table(t, r, c, i, name, dtype=_F32):
+    """pointer of a contiguous [r, c] tensor on device i (None: null)"""
+    if t is not None and t.shape != (r, c): _refuse(f"{name}: a tensor of shape {(r, c)} is wanted, not {tuple(t.shape)}")
+    return _vec(t, r * c, i, name, dtype)
+def _workspace(n, i):
+    """n bytes on device i, of the current stream (or of the graph that is being captured); None for none"""
+    return torch.empty(n, dtype=torch.uint8, device=_devices[i]) if n else None
+def _run(i, f, *args):
+    """f(*args, stream) on device i and its current stream"""
+    if i == _current_device(): status = f(*args, _raw_stream(i))
     else:
-        with torch.cuda.device(i): _l.check(f(*args, _raw_stream(i)))
+        with torch.cuda.device(i): status = f(*args, _raw_stream(i))
+    if status: _l.check(status)
 
 class CuMatrix:
     def __init__(self, t):
@@ -114,21 +127,19 @@ def DiffNormalizePerRow(in_value, out_deriv, target_rms, add_log_stddev, in_deri
 def LayerNormPerRow(inp, scale, offset, eps, out, mean=None, inv_std=None):
     """Layer norm: out = (inp - mean) inv_std scale + offset row by row, inv_std = 1 / sqrt(var + eps).  inp, out: matrices of one type (float32, float16, bfloat16), out may be inp;
     scale, offset: float32 vectors of the row length or None; mean, inv_std: float32 vectors of the number of rows that receive the statistics DiffLayerNormPerRow takes, or None."""
-    x, ldx = _rows(inp, "inp"); y, ldy = _like_rows(out, x, "out"); r, c = x.shape
+    x = _rows(inp, "inp"); dt, px, ldx, r, c, i = x; y, ldy = _like_rows(out, x, "out")
     if not 0.0 <= eps < float("inf"): _refuse(f"eps: {eps}")
-    _run(x, _l.load().k3_layer_norm_forward, _DTYPES[x.dtype], x.data_ptr(), ldx, _vec(scale, (c,), x, "scale"), _vec(offset, (c,), x, "offset"), eps, y.data_ptr(), ldy,
-         _vec(mean, (r,), x, "mean"), _vec(inv_std, (r,), x, "inv_std"), r, c)
+    _run(i, _l.load().k3_layer_norm_forward, dt, px, ldx, _vec(scale, c, i, "scale"), _vec(offset, c, i, "offset"), eps, y, ldy, _vec(mean, r, i, "mean"), _vec(inv_std, r, i, "inv_std"), r, c)
 def DiffLayerNormPerRow(in_value, out_deriv, scale, mean, inv_std, in_deriv=None, scale_deriv=None, offset_deriv=None, accumulate=False):
     """The backward pass of LayerNormPerRow from its input, its kept statistics and the derivative with respect to its output.  in_deriv (may be out_deriv or in_value) is overwritten;
     scale_deriv, offset_deriv (float32 vectors) are overwritten, or added to with accumulate.  What is None is not computed."""
-    x, ldx = _rows(in_value, "in_value"); g, ldg = _like_rows(out_deriv, x, "out_deriv"); r, c = x.shape
+    x = _rows(in_value, "in_value"); dt, px, ldx, r, c, i = x; g, ldg = _like_rows(out_deriv, x, "out_deriv")
     if mean is None or inv_std is None: _refuse("mean, inv_std: the statistics of the forward pass are wanted")
     d, ldd = (None, c) if in_deriv is None else _like_rows(in_deriv, x, "in_deriv")
-    L = _l.load(); ws = None
-    if scale_deriv is not None or offset_deriv is not None: ws = torch.empty(L.k3_layer_norm_backward_workspace(r, c), dtype=torch.uint8, device=x.device)
-    _run(x, L.k3_layer_norm_backward, _DTYPES[x.dtype], x.data_ptr(), ldx, g.data_ptr(), ldg, _vec(scale, (c,), x, "scale"), _vec(mean, (r,), x, "mean"), _vec(inv_std, (r,), x, "inv_std"),
-         None if d is None else d.data_ptr(), ldd, _vec(scale_deriv, (c,), x, "scale_deriv"), _vec(offset_deriv, (c,), x, "offset_deriv"), int(accumulate),
-         None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), r, c)
+    L = _l.load(); ws = None; n = 0
+    if scale_deriv is not None or offset_deriv is not None: n = L.k3_layer_norm_backward_workspace(r, c); ws = _workspace(n, i)
+    _run(i, L.k3_layer_norm_backward, dt, px, ldx, g, ldg, _vec(scale, c, i, "scale"), _vec(mean, r, i, "mean"), _vec(inv_std, r, i, "inv_std"), d, ldd,
+         _vec(scale_deriv, c, i, "scale_deriv"), _vec(offset_deriv, c, i, "offset_deriv"), 1 if accumulate else 0, ws.data_ptr() if n else None, n, r, c)
 
 class CuRand:
     """CuRand<BaseFloat> (cudamatrix/cu-rand.h:31-64) over k3_mat_set_rand: one seed per object, the counter position advances by what each fill consumes"""
