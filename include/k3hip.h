@@ -576,6 +576,19 @@ int64_t k3_layer_norm_backward_workspace(int32_t rows, int32_t cols);
 int k3_layer_norm_backward(int32_t dtype, const void *d_x, int64_t ldx, const void *d_dy, int64_t lddy, const float *d_scale, const float *d_mean, const float *d_inv_std,
                            void *d_dx, int64_t lddx, float *d_dscale, float *d_doffset, int32_t accumulate, void *d_workspace, int64_t workspace_bytes,
                            int32_t rows, int32_t cols, void *stream);
+/* An affine layer in half precision (dtype K3_F16 or K3_BF16): pre = x W^T + bias, y = act(pre) + residual, x [rows x inner], W [cols x inner] (AffineComponent's linear_params),
+ * d_bias float32 [cols] (null: 0), d_residual [rows x cols] (null: none; y may be it).  d_pre (null: not kept) receives pre as the backward pass takes it.  Products are summed in float32 and
+ * a result is rounded once.  Stands beside k3_mat_add_mat_mat, which is float32 and has no epilogue.  Workspace (16-byte aligned): k3_affine_forward_workspace. */
+typedef enum { K3_ACT_NONE = 0, K3_ACT_RELU = 1, K3_ACT_SIGMOID = 2, K3_ACT_TANH = 3, K3_ACT_SWISH = 4 /* z sigmoid(z) */, K3_ACT_GELU = 5 /* z (1 + erf(z / sqrt 2)) / 2 */ } k3_activation;
+int64_t k3_affine_forward_workspace(int32_t rows, int32_t inner, int32_t cols);
+int k3_affine_forward(int32_t dtype, int32_t act, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const float *d_bias, const void *d_residual, int64_t ldr, void *d_y,
+                      int64_t ldy, void *d_pre, int64_t ldp, void *d_workspace, int64_t workspace_bytes, int32_t rows, int32_t inner, int32_t cols, void *stream);
+/* Its derivatives from dy: dz = dy act'(pre) (d_pre not read for K3_ACT_NONE), d_dx = dz W and d_dw = dz^T x (of the matrices' type), d_db [cols] = the sum of dz over the rows (float32);
+ * each may be null (not wanted), and what is given is overwritten.  (The residual's derivative is dy itself.)  Where there is an activation, dz is rounded to the matrices' type for the two
+ * products, not for d_db.  Sums are taken in a fixed order.  rows = 0 clears d_dw and d_db.  Workspace (16-byte aligned): k3_affine_backward_workspace. */
+int64_t k3_affine_backward_workspace(int32_t act, int32_t rows, int32_t inner, int32_t cols);
+int k3_affine_backward(int32_t dtype, int32_t act, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_pre, int64_t ldp, const void *d_dy, int64_t lddy,
+                       void *d_dx, int64_t lddx, void *d_dw, int64_t lddw, float *d_db, void *d_workspace, int64_t workspace_bytes, int32_t rows, int32_t inner, int32_t cols, void *stream);
 /* Scores of the rows of a network's output z: the log-probability log q_y of one label y per row under the row's softmax, the row's entropy -sum q log q, and its num_alternatives
  * (0 .. 64) most probable columns with their log-probabilities, best first, equal ones by column.  Stands beside CuMatrixBase::LogSoftMaxPerRow (cudamatrix/cu-matrix.h:334), without
  * the matrix of log-probabilities.  d_labels [rows] (a label outside 0 .. cols - 1, -1 for instance, = none: its log-probability is 0); every output may be null: d_log_prob, d_entropy

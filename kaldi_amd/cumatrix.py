@@ -141,6 +141,44 @@ def DiffLayerNormPerRow(in_value, out_deriv, scale, mean, inv_std, in_deriv=None
     _run(i, L.k3_layer_norm_backward, dt, px, ldx, g, ldg, _vec(scale, c, i, "scale"), _vec(mean, r, i, "mean"), _vec(inv_std, r, i, "inv_std"), d, ldd,
          _vec(scale_deriv, c, i, "scale_deriv"), _vec(offset_deriv, c, i, "offset_deriv"), 1 if accumulate else 0, ws.data_ptr() if n else None, n, r, c)
 
+ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2, "tanh": 3, "swish": 4, "gelu": 5}      # k3_activation
+def _half_rows(m, name):
+    x = _rows(m, name)
+    if x[0] == 0: _refuse(f"{name}: float16 or bfloat16 is wanted (float32 products: CuMatrix.AddMatMat)")
+    return x
+def _rows_of(m, r, c, x, name):
+    """a matrix of r x c of x's type and device (None: none): (pointer, leading dimension)"""
+    if m is None: return None, c
+    y = _rows(m, name)
+    if y[3] != r or y[4] != c or y[0] != x[0] or y[5] != x[5]: _refuse(f"{name}: {y[3]} x {y[4]} of type {y[0]} on device {y[5]}: {r} x {c} of type {x[0]} on device {x[5]} is wanted")
+    return y[1], y[2]
+def AffinePerRow(inp, linear_params, bias_params, activation, residual, out, pre_activation=None):
+    """An affine layer in float16 or bfloat16: out = activation(inp linear_params^T + bias_params) + residual.  inp [rows, inner], linear_params [cols, inner]; bias_params: float32 vector of
+    cols or None; activation: one of ACTIVATIONS; residual [rows, cols] or None (out may be it); pre_activation [rows, cols] receives inp linear_params^T + bias_params, which
+    DiffAffinePerRow takes, or None."""
+    x = _half_rows(inp, "inp"); dt, px, ldx, r, k, i = x; act = ACTIVATIONS.get(activation)
+    if act is None: _refuse(f"activation: {activation!r} is none of {', '.join(ACTIVATIONS)}")
+    wt, pw, ldw, c, wk, wi = _rows(linear_params, "linear_params")
+    if wt != dt or wk != k or wi != i: _refuse(f"linear_params: {c} x {wk} of type {wt} on device {wi} does not go with an input of {k} columns of type {dt} on device {i}")
+    res, ldr = _rows_of(residual, r, c, x, "residual")
+    if out is None: _refuse("out: a matrix is wanted")
+    y, ldy = _rows_of(out, r, c, x, "out"); pre, ldp = _rows_of(pre_activation, r, c, x, "pre_activation")
+    L = _l.load(); n = L.k3_affine_forward_workspace(r, k, c); ws = _workspace(n, i)
+    _run(i, L.k3_affine_forward, dt, act, px, ldx, pw, ldw, _vec(bias_params, c, i, "bias_params"), res, ldr, y, ldy, pre, ldp, ws.data_ptr() if n else None, n, r, k, c)
+def DiffAffinePerRow(in_value, linear_params, pre_activation, activation, out_deriv, in_deriv=None, linear_params_deriv=None, bias_params_deriv=None):
+    """The backward pass of AffinePerRow from its input, its weights, the kept pre_activation (None for the activation "none") and the derivative with respect to its output, which is the
+    residual's derivative too.  in_deriv, linear_params_deriv (matrices) and bias_params_deriv (float32 vector) are overwritten; what is None is not computed."""
+    x = _half_rows(in_value, "in_value"); dt, px, ldx, r, k, i = x; act = ACTIVATIONS.get(activation)
+    if act is None: _refuse(f"activation: {activation!r} is none of {', '.join(ACTIVATIONS)}")
+    wt, pw, ldw, c, wk, wi = _rows(linear_params, "linear_params")
+    if wt != dt or wk != k or wi != i: _refuse(f"linear_params: {c} x {wk} of type {wt} on device {wi} does not go with an input of {k} columns of type {dt} on device {i}")
+    if out_deriv is None: _refuse("out_deriv: a matrix is wanted")
+    if pre_activation is None and act: _refuse("pre_activation: what the forward pass kept is wanted")
+    pre, ldp = _rows_of(pre_activation, r, c, x, "pre_activation"); g, ldg = _rows_of(out_deriv, r, c, x, "out_deriv")
+    dx, lddx = _rows_of(in_deriv, r, k, x, "in_deriv"); dw, lddw = _rows_of(linear_params_deriv, c, k, x, "linear_params_deriv")
+    L = _l.load(); n = L.k3_affine_backward_workspace(act, r, k, c); ws = _workspace(n, i)
+    _run(i, L.k3_affine_backward, dt, act, px, ldx, pw, ldw, pre, ldp, g, ldg, dx, lddx, dw, lddw, _vec(bias_params_deriv, c, i, "bias_params_deriv"), ws.data_ptr() if n else None, n, r, k, c)
+
 class CuRand:
     """CuRand<BaseFloat> (cudamatrix/cu-rand.h:31-64) over k3_mat_set_rand: one seed per object, the counter position advances by what each fill consumes"""
     def __init__(self, seed=0): self.seed, self.offset, self._L = int(seed), 0, _l.load()

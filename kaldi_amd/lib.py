@@ -160,6 +160,10 @@ def load():
     L.k3_layer_norm_forward.argtypes = [i32, vp, i64, vp, vp, f32, vp, i64, vp, vp, i32, i32, vp]
     L.k3_layer_norm_backward_workspace.argtypes = [i32, i32]; L.k3_layer_norm_backward_workspace.restype = i64
     L.k3_layer_norm_backward.argtypes = [i32, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, i32, vp, i64, i32, i32, vp]
+    L.k3_affine_forward_workspace.argtypes = [i32, i32, i32]; L.k3_affine_forward_workspace.restype = i64
+    L.k3_affine_forward.argtypes = [i32, i32, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, vp]
+    L.k3_affine_backward_workspace.argtypes = [i32, i32, i32, i32]; L.k3_affine_backward_workspace.restype = i64
+    L.k3_affine_backward.argtypes = [i32, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i64, i32, i32, i32, vp]
     L.k3_label_logprobs_workspace.argtypes = [i32, i32, i32, i32]; L.k3_label_logprobs_workspace.restype = i64
     L.k3_label_logprobs.argtypes = [i32, vp, i64, vp, vp, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp]
     L.k3_label_logprobs_deriv.argtypes = [i32, vp, i64, vp, vp, vp, vp, vp, vp, i64, i32, i32, vp]

@@ -46,10 +46,30 @@ def test_distillation_entry_point():
     need = L.k3_distill_workspace(0, 4, 200000, 3, 1); assert need > 0 and L.k3_distill_workspace(0, 4, 6024, 3, 1) == 0
     refused(f(cols=200000, ld=200000, ldd=200000, ws=P, nb=need - 1), "workspace"); refused(f(cols=200000, ld=200000, ldd=200000), "workspace"); refused(f(cols=200000, ld=200000, ldd=200000, ws=P + 8, nb=need), "workspace")
 
+def test_affine_entry_points():
+    L = _l.load()
+    need = L.k3_affine_forward_workspace(4, 4096, 8); assert need > 0
+    f = lambda dtype=1, act=0, x=P, ldx=4096, w=P, ldw=4096, r=None, ldr=8, y=P, ldy=8, pre=None, ldp=8, ws=P, n=need, rows=4, inner=4096, cols=8: L.k3_affine_forward(dtype, act, x, ldx, w, ldw, None, r, ldr, y, ldy, pre, ldp, ws, n, rows, inner, cols, None)  # noqa: E731
+    for d in (0, 3, -1): refused(f(dtype=d), "float16 and bfloat16")
+    refused(f(act=6), "activation"); refused(f(act=-1), "activation")
+    for k in ("ldx", "ldw", "ldy"): refused(f(**{k: 7}), "bad argument")
+    refused(f(r=P, ldr=7), "bad argument"); refused(f(pre=P, ldp=7), "bad argument"); refused(f(rows=-1), "bad argument"); refused(f(inner=0), "bad argument"); refused(f(cols=0), "bad argument")
+    refused(f(inner=1 << 21, ldx=1 << 21, ldw=1 << 21), "too large"); refused(f(rows=(1 << 31) - 1, cols=4096, ldy=4096), "too large")
+    for k in ("x", "w", "y"): refused(f(**{k: None}), "null")
+    refused(f(ws=None), "workspace"); refused(f(n=need - 1), "workspace"); refused(f(ws=P + 4), "workspace"); assert f(rows=0) == 0
+    need = L.k3_affine_backward_workspace(1, 4, 4096, 8); assert need > 0
+    b = lambda dtype=1, act=1, x=P, ldx=4096, w=P, ldw=4096, pre=P, ldp=8, dy=P, lddy=8, dx=P, lddx=4096, dw=P, lddw=4096, ws=P, n=need, rows=4, inner=4096, cols=8: L.k3_affine_backward(dtype, act, x, ldx, w, ldw, pre, ldp, dy, lddy, dx, lddx, dw, lddw, P, ws, n, rows, inner, cols, None)  # noqa: E731
+    refused(b(dtype=0), "float16 and bfloat16"); refused(b(act=9), "activation")
+    for k in ("ldx", "ldw", "ldp", "lddy", "lddx", "lddw"): refused(b(**{k: 7}), "bad argument")
+    refused(b(rows=-1), "bad argument"); refused(b(inner=0), "bad argument"); refused(b(cols=0), "bad argument"); refused(b(inner=1 << 21, ldx=1 << 21, ldw=1 << 21, lddx=1 << 21, lddw=1 << 21), "too large")
+    for k in ("x", "w", "pre", "dy"): refused(b(**{k: None}), "null")
+    refused(b(ws=None), "workspace"); refused(b(n=need - 1), "workspace"); refused(b(ws=P + 4), "workspace")
+
 def test_matrices_that_are_no_rows_on_a_gpu():
     from kaldi_amd import cumatrix as cm, objective as ob
     t = torch.zeros(4, 8)
     for bad, word in ((t, "GPU"), (torch.zeros(4), "matrix"), (torch.zeros(4, 8, dtype=torch.float64), "matrix"), (torch.zeros(4, 8, dtype=torch.int32), "matrix"), ("x", "matrix")):
         with pytest.raises(K3Error, match=word): cm.LayerNormPerRow(bad, None, None, 1e-5, bad)
         with pytest.raises(K3Error, match=word): ob.LabelLogProbs(bad, None)
+        with pytest.raises(K3Error, match=word): cm.AffinePerRow(bad, bad, None, "none", None, bad)
         with pytest.raises(K3Error, match=word): ob.ComputeDistillObjfAndDeriv(ob.DistillationOptions(), bad, bad, bad, None, None)
