@@ -13,24 +13,39 @@ using namespace k3;
 
 enum { kNone = K3_ACT_NONE, kRelu = K3_ACT_RELU, kSigmoid = K3_ACT_SIGMOID, kTanh = K3_ACT_TANH, kSwish = K3_ACT_SWISH, kGelu = K3_ACT_GELU };
 
-__device__ inline float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+__device__ inline float exp_fast(float z) { return __builtin_amdgcn_exp2f(z * 1.44269504088896340736f); }
+__device__ inline float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_fast(-z)); }
+// 1 - 2 / (e^2z + 1), and its series to z^5 where that would cancel
+__device__ inline float tanh_fast(float z) {
+  const float q = z * z;
+  return fabsf(z) < 0.1f ? z * (1.0f + q * (-0.33333333f + q * 0.13333333f)) : 1.0f - 2.0f * __builtin_amdgcn_rcpf(exp_fast(2.0f * z) + 1.0f);
+}
+// erf(z / sqrt 2) to 1.5e-7 (Abramowitz and Stegun, 7.1.26), with e = exp(-z^2 / 2) for who needs it too
+__device__ inline float erf_half(float z, float &e) {
+  const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+  e = exp_fast(-0.5f * z * z);
+  const float r = 1.0f - t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * e;
+  return z < 0.0f ? -r : r;
+}
+// (-inf goes in as a number whose exponential is 0 all the same: 0 times it is 0)
 __device__ inline float activation(int act, float z) {
   switch (act) {
     case kRelu: return z < 0.0f ? 0.0f : z;      // (a NaN stays one)
     case kSigmoid: return sigmoid(z);
-    case kTanh: return tanhf(z);
-    case kSwish: return z * sigmoid(z);
-    case kGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case kTanh: return tanh_fast(z);
+    case kSwish: z = z < -1e4f ? -1e4f : z; return z * sigmoid(z);
+    case kGelu: { float e; z = z < -1e4f ? -1e4f : z; return 0.5f * z * (1.0f + erf_half(z, e)); }
     default: return z;
   }
 }
 __device__ inline float slope(int act, float z) {
+  z = z < -1e4f ? -1e4f : z > 1e4f ? 1e4f : z;
   switch (act) {
     case kRelu: return z > 0.0f ? 1.0f : z == z ? 0.0f : z;
     case kSigmoid: { const float s = sigmoid(z); return s * (1.0f - s); }
-    case kTanh: { const float s = tanhf(z); return 1.0f - s * s; }
+    case kTanh: { const float s = tanh_fast(z); return 1.0f - s * s; }
     case kSwish: { const float s = sigmoid(z); return s * (1.0f + z * (1.0f - s)); }
-    case kGelu: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    case kGelu: { float e; const float f = erf_half(z, e); return 0.5f * (1.0f + f) + z * 0.39894228040143268f * e; }
     default: return 1.0f;
   }
 }
@@ -50,81 +65,100 @@ typedef __attribute__((address_space(3))) s4 lds_s4;
 
 struct Epilogue {
   void *c; long long ldc;
-  float *partial;                  // the contraction in parts: float32 planes [part][M][N], joined by k3_affine_join_kernel
   const float *bias;               // [N] or null
   const void *residual; long long ldr;
   void *pre; long long ldp;
   int act;
 };
-struct Product { const void *a; long long lda; const void *b; long long ldb; int m, n, k; int tiles_m, tiles_n, parts, steps_per_part; Epilogue e; };
+// C [m x n] over k contraction steps, in tiles.  The first `whole` tiles are one workgroup's each; those behind them (what would leave most of the chip idle) are `parts` workgroups' each, of
+// steps_per_part LDS tiles of the contraction, whose float32 sums go to partial [tile][part][BM][BN] and are joined by k3_affine_join_kernel.
+struct Product { const void *a; long long lda; const void *b; long long ldb; int m, n, k; int tiles_m, tiles_n, whole, parts, steps_per_part; float *partial; Epilogue e; };
 
-constexpr int BK = 64;             // contraction steps per LDS tile
+typedef float f8 __attribute__((ext_vector_type(8)));
 
-// 4 consecutive outputs of one row
-template <typename T> __device__ inline void finish(const Epilogue &e, long long row, int col, int n, f4 v) {
-  typedef T t4 __attribute__((ext_vector_type(4), aligned(2)));
-  const T *res = e.residual ? (const T *)e.residual + row * e.ldr + col : nullptr;
-  T *c = (T *)e.c + row * e.ldc + col, *pre = e.pre ? (T *)e.pre + row * e.ldp + col : nullptr;
-  if (n - col >= 4) {
-    typedef float fu __attribute__((ext_vector_type(4), aligned(4)));
-    if (e.bias) v += *(const fu *)(e.bias + col);
-    if (pre) *(t4 *)pre = __builtin_convertvector(v, t4);
-    if (e.act != kNone)
+// 8 consecutive outputs of a row, `valid` of which exist
+template <typename T> __device__ inline void finish(const Epilogue &e, long long row, int col, int valid, f8 v) {
+  typedef typename Chunk<T>::type t8;
+  t8 res;
+  if (e.residual) res = load_chunk((const T *)e.residual + row * e.ldr, col, valid);
+  if (e.bias) {
+    float b[8];
+    load_params<8>(e.bias, col, valid, 0.0f, b);
 #pragma unroll
-      for (int j = 0; j < 4; j++) v[j] = activation(e.act, v[j]);
-    if (res) v += __builtin_convertvector(*(const t4 *)res, f4);
-    *(t4 *)c = __builtin_convertvector(v, t4);
-  } else
+    for (int j = 0; j < 8; j++) v[j] += b[j];
+  }
+  if (e.pre) store_chunk((T *)e.pre + row * e.ldp, col, valid, __builtin_convertvector(v, t8));
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (col + j < n) {
-        float u = v[j] + (e.bias ? e.bias[col + j] : 0.0f);
-        if (pre) pre[j] = (T)u;
-        u = activation(e.act, u);
-        c[j] = (T)(res ? u + to_f32(res[j]) : u);
-      }
+  for (int j = 0; j < 8; j++) v[j] = activation(e.act, v[j]);
+  if (e.residual) v += __builtin_convertvector(res, f8);
+  store_chunk((T *)e.c + row * e.ldc, col, valid, __builtin_convertvector(v, t8));
+}
+// U times 8 outputs of the same columns, all of which exist, in rows row0 + u step below m: no activation or ReLU, and what is read for all of them on its way before the first is finished
+template <typename T, int U, typename V> __device__ inline void finish_rows(const Epilogue &e, long long row0, int step, int m, int col, V value) {
+  typedef typename Chunk<T>::type t8;
+  t8 res[U];
+  if (e.residual)
+#pragma unroll
+    for (int u = 0; u < U; u++) res[u] = *(const t8 *)((const T *)e.residual + min(row0 + u * step, m - 1ll) * e.ldr + col);
+  float b[8] = {};
+  if (e.bias) load_params<8>(e.bias, col, 8, 0.0f, b);
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const long long row = row0 + u * step;
+    f8 v = value(u);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] += b[j];
+    if (row < m) {
+      if (e.pre) *(t8 *)((T *)e.pre + row * e.ldp + col) = __builtin_convertvector(v, t8);
+      if (e.act == kRelu)
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = activation(kRelu, v[j]);
+      if (e.residual) v += __builtin_convertvector(res[u], f8);
+      *(t8 *)((T *)e.c + row * e.ldc + col) = __builtin_convertvector(v, t8);
+    }
+  }
 }
 
 // what the wavefront's lanes have written to LDS before it they read after it
 __device__ inline void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 
-// An LDS tile of ROWS rows (of the operand's output index) by BK contraction steps, in chunks of 8 elements.  ACROSS false: [row][8 chunks], a row's chunk c at c ^ (row / 2 % 8): 16
-// lanes that read the same chunk of 16 rows touch every 16-byte column of two LDS rows once.  ACROSS true (the contraction index is the memory row): [step][ROWS / 8 chunks], pairs
-// of chunks (16 rows of the operand) exchanged by an XOR with bits of the step that differ among the lanes of one transposing read.
-template <int ROWS, bool ACROSS> struct Tile {
-  static constexpr int kChunks = ROWS * BK / 8, kBytes = kChunks * 16;
-  static __device__ inline int spread(int k) {
-    return ROWS >= 128 ? (k & 3) | (k >> 3 & 1) << 2 : ROWS == 64 ? (k >> 1 & 1) | (k >> 3 & 1) << 1 : k >> 3 & 1;
-  }
-  // LDS position p (in chunks) -> row / step and chunk of the operand
+// An LDS tile of ROWS rows (of the operand's output index) by BK contraction steps, in chunks of 8 elements and blocks of 64 of them (what a wavefront loads at once).
+// ACROSS false: [row][BK / 8 chunks], a row's chunk c at c ^ a function of the row such that 16 lanes that read the same chunk of 16 rows touch every 16-byte column of 256 bytes once.
+// ACROSS true (the contraction index is the memory row): a block holds 512 / ROWS steps of all rows; the 4 steps that 16 lanes read at once with one transposing read lie in the 4 blocks of
+// a set, which are 32 bytes more than their size apart and so start in different banks, and neighbouring groups of lanes read from different sets (or from halves of a block 128 bytes
+// apart).  (No XOR: a lane's reads of all its rows differ by constants alone.)
+template <int ROWS, int BK, bool ACROSS> struct Tile {
+  static constexpr int kChunks = ROWS * BK / 8, CH = BK / 8, kBlock = ACROSS ? 1056 : 1024, kBytes = kChunks / 64 * kBlock, SETS = kChunks / 256;
+  static __device__ inline int spread(int row) { return row / (16 / CH) & (CH - 1); }
+  // chunk p of the tile in the order of LDS -> row / step and chunk of the operand
   static __device__ inline void source(int p, int &major, int &chunk) {
-    if (ACROSS) {
-      major = p / (ROWS / 8);
-      const int c = p % (ROWS / 8);
-      chunk = ((c >> 1) ^ spread(major)) << 1 | (c & 1);
+    if constexpr (ACROSS) {
+      const int block = p / 64, slot = p % 64 / (ROWS / 8);
+      major = (slot / 2 * SETS + block / 4) * 8 + slot % 2 * 4 + block % 4;
+      chunk = p % (ROWS / 8);
     } else {
-      major = p / 8;
-      chunk = (p % 8) ^ (major >> 1 & 7);
+      major = p / CH;
+      chunk = (p % CH) ^ spread(major);
     }
   }
   // the fragment of 16 rows from `row` (a multiple of 16) and the contraction steps 32 ks + 8 (lane / 16) ..
   template <typename T> static __device__ inline typename Half<T>::frag fragment(const char *tile, int row, int ks, int lane) {
     if constexpr (ACROSS) {
-      const int k = 32 * ks + 8 * (lane >> 4) + (lane & 15) / 4;
-      const char *p = tile + k * (ROWS * 2) + ((row >> 4) ^ spread(k)) * 32 + (lane & 3) * 8;
-      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 4 * ROWS * 2));
+      const int set = SETS == 8 ? 4 * ks + (lane >> 4) : (lane >> 4) % SETS, slot = SETS == 8 ? 0 : 2 * ((4 * ks + (lane >> 4)) / SETS), block = set * 4 + (lane & 15) / 4;
+      const char *p = tile + block * kBlock + slot * (ROWS * 2) + (lane & 3) * 8 + row * 2;
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + ROWS * 2));
       return __builtin_bit_cast(typename Half<T>::frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
       const int r = row + (lane & 15), c = 4 * ks + (lane >> 4);
-      return *(const typename Half<T>::frag *)(tile + r * 128 + (c ^ (r >> 1 & 7)) * 16);
+      return *(const typename Half<T>::frag *)(tile + r * (BK * 2) + (c ^ spread(lane & 15)) * 16);
     }
   }
 };
 
 // One operand's way into LDS for a workgroup of THREADS.  direct: global memory to LDS without registers (16-byte aligned rows; chunks that begin behind the operand's last row are read from
 // its first one, and their products never stored); otherwise through registers, with zeros where the operand ends, at any alignment.
-template <typename T, int ROWS, bool ACROSS, int THREADS> struct Loader {
-  using L = Tile<ROWS, ACROSS>;
+template <typename T, int ROWS, int BK, bool ACROSS, int THREADS> struct Loader {
+  using L = Tile<ROWS, BK, ACROSS>;
   static constexpr int N = L::kChunks / THREADS;
   typedef T chunk __attribute__((ext_vector_type(8)));
   const T *base; long long ld; int row0, rows, k;      // the operand, its first row in this tile, its number of rows, and the contraction's length
@@ -141,7 +175,7 @@ template <typename T, int ROWS, bool ACROSS, int THREADS> struct Loader {
   __device__ inline void direct(unsigned lds) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const unsigned to = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x / 64 * N + i) * 1024);
+      const unsigned to = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x / 64 * N + i) * L::kBlock);
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)at[i], (__attribute__((address_space(3))) void *)(unsigned long long)to, 16, 0, 0);
       at[i] += ACROSS ? BK * ld : BK;
     }
@@ -162,89 +196,155 @@ template <typename T, int ROWS, bool ACROSS, int THREADS> struct Loader {
   }
   static __device__ inline void store(char *tile, const chunk (&v)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; i++) *(chunk *)(tile + ((threadIdx.x / 64 * N + i) * 64 + (threadIdx.x & 63)) * 16) = v[i];
+    for (int i = 0; i < N; i++) *(chunk *)(tile + (threadIdx.x / 64 * N + i) * L::kBlock + (threadIdx.x & 63) * 16) = v[i];
   }
 };
 
-// BM x BN outputs per workgroup of WM x WN wavefronts; two LDS tiles per operand, the next one on its way while the present one is multiplied.
+// a barrier behind which the LDS loads that the workgroup's wavefronts issued are there and their LDS reads are done (raw, so that nothing else is waited for); no memory operation crosses it
+__device__ inline void arrive() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// tiles in panels of 8 columns of them, row after row within a panel: any 32 neighbours (what an XCD works on at once) share few rows and columns of the operands
+__device__ inline void place(const Product &p, int tile, int &tm, int &tn) {
+  const int panel = tile / (8 * p.tiles_m), rest = tile - panel * 8 * p.tiles_m, width = min(8, p.tiles_n - panel * 8);
+  tm = rest / width;
+  tn = panel * 8 + rest - tm * width;
+}
+
+// BM x BN outputs per workgroup of WM x WN wavefronts, over LDS tiles of 64 contraction steps, two of them: one is loaded while the other is multiplied.  PIPED (the size of which a compute
+// unit holds one workgroup): a tile is two halves of 32 steps for the matrix instructions, and the fragments of a half are read from LDS among the instructions of the half before it, those of the next tile's first half too: the one barrier per
+// tile stands between the halves, where every wavefront has read all of this tile (which the loads issued behind the barrier then overwrite) and the next one has arrived.
 template <typename T, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product p) {
-  constexpr int THREADS = 64 * WM * WN, MI = BM / WM / 16, NI = BN / WN / 16;
-  using TA = Tile<BM, A_ACROSS>;
-  using TB = Tile<BN, B_ACROSS>;
-  __shared__ __attribute__((aligned(1024))) char lds[2][TA::kBytes + TB::kBytes];
+  constexpr int THREADS = 64 * WM * WN, MI = BM / WM / 16, NI = BN / WN / 16, BK = 64;
+  constexpr bool PIPED = BM == 256;
+  using TA = Tile<BM, BK, A_ACROSS>;
+  using TB = Tile<BN, BK, B_ACROSS>;
+  using LA = Loader<T, BM, BK, A_ACROSS, THREADS>;
+  using LB = Loader<T, BN, BK, B_ACROSS, THREADS>;
+  constexpr int kStage = TA::kBytes + TB::kBytes;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
-  // workgroups go round the 8 XCDs: each XCD takes a run of neighbouring tiles (columns fastest), which share operands in its L2
-  const int tiles = p.tiles_m * p.tiles_n, per = tiles / 8, extra = tiles % 8, x = blockIdx.x % 8, i8 = blockIdx.x / 8;
-  const int tile = x * per + min(x, extra) + i8, tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
-  const int first = blockIdx.y * p.steps_per_part * BK, end = min(p.k, first + p.steps_per_part * BK), whole = (end - first) / BK, steps = (end - first + BK - 1) / BK;
-  Loader<T, BM, A_ACROSS, THREADS> la{(const T *)p.a, p.lda, tm * BM, p.m, p.k};
-  Loader<T, BN, B_ACROSS, THREADS> lb{(const T *)p.b, p.ldb, tn * BN, p.n, p.k};
-  const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char *)lds[0], stage = TA::kBytes + TB::kBytes;
+  // workgroups go round the 8 XCDs: each XCD takes a run of neighbouring tiles, which share operands in its L2; so do the parts of the last tiles
+  const bool split = (int)blockIdx.x >= p.whole;
+  const int units = split ? (p.tiles_m * p.tiles_n - p.whole) * p.parts : p.whole, u = split ? blockIdx.x - p.whole : blockIdx.x;
+  const int per = units / 8, extra = units % 8, x = u % 8, unit = x * per + min(x, extra) + u / 8;
+  const int tile = split ? p.whole + unit / p.parts : unit, part = split ? unit % p.parts : 0;
+  int tm, tn;
+  place(p, tile, tm, tn);
+  const int first = split ? part * p.steps_per_part * BK : 0, end = split ? min(p.k, first + p.steps_per_part * BK) : p.k;
+  const int direct = DIRECT ? max(end - first, 0) / BK : 0, steps = (max(end - first, 0) + BK - 1) / BK;
+  LA la{(const T *)p.a, p.lda, tm * BM, p.m, p.k};
+  LB lb{(const T *)p.b, p.ldb, tn * BN, p.n, p.k};
   f4 acc[MI][NI] = {};
-  const auto multiply = [&](const char *ta) {
-    const char *tb = ta + TA::kBytes;
+  typedef typename Half<T>::frag frag;
+  const auto read = [&](const char *ta, int ks, frag (&a)[MI], frag (&b)[NI]) {
 #pragma unroll
-    for (int ks = 0; ks < BK / 32; ks++) {
-      typename Half<T>::frag a[MI], b[NI];
+    for (int j = 0; j < NI; j++) b[j] = TB::template fragment<T>(ta + TA::kBytes, wn * (BN / WN) + j * 16, ks, lane);
 #pragma unroll
-      for (int j = 0; j < NI; j++) b[j] = TB::template fragment<T>(tb, wn * (BN / WN) + j * 16, ks, lane);
+    for (int i = 0; i < MI; i++) a[i] = TA::template fragment<T>(ta, wm * (BM / WM) + i * 16, ks, lane);
+  };
+  const auto multiply = [&](const frag (&a)[MI], const frag (&b)[NI]) {
 #pragma unroll
-      for (int i = 0; i < MI; i++) a[i] = TA::template fragment<T>(ta, wm * (BM / WM) + i * 16, ks, lane);
+    for (int i = 0; i < MI; i++)
 #pragma unroll
-      for (int i = 0; i < MI; i++)
+      for (int j = 0; j < NI; j++) Half<T>::mfma(b[j], a[i], acc[i][j]);      // (n, m): a lane ends with 4 consecutive n of one m
+  };
+  // the order of a half: its loads and LDS reads spread over the first part of its matrix instructions
+  constexpr int READS = (A_ACROSS ? 2 : 1) * MI + (B_ACROSS ? 2 : 1) * NI;
+  const auto interleave = [&](auto loads) {
+    constexpr int L = decltype(loads)::value, PER = MI * NI / (READS + L) > 0 ? MI * NI / (READS + L) : 1;
 #pragma unroll
-        for (int j = 0; j < NI; j++) Half<T>::mfma(b[j], a[i], acc[i][j]);      // (n, m): a lane ends with 4 consecutive n of one m
+    for (int i = 0; i < READS; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
     }
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, MI * NI, 0);
   };
   if constexpr (DIRECT) {
-    la.start(first);
-    lb.start(first);
-    if (whole) {
-      la.direct(lds0);
-      lb.direct(lds0 + TA::kBytes);
-      __syncthreads();
-    }
-    for (int s = 0; s < whole; s++) {
-      if (s + 1 < whole) {
-        la.direct(lds0 + ((s + 1) & 1) * stage);
-        lb.direct(lds0 + ((s + 1) & 1) * stage + TA::kBytes);
+    if (direct) {
+      const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char *)lds;
+      la.start(first);
+      lb.start(first);
+      const auto issue = [&](int s) {
+        la.direct(lds0 + (s & 1) * kStage);
+        lb.direct(lds0 + (s & 1) * kStage + TA::kBytes);
+      };
+      issue(0);
+      if constexpr (PIPED) {
+        frag a0[MI], b0[NI], a1[MI], b1[NI];
+        __syncthreads();
+        if (direct > 1) issue(1);
+        read(lds, 0, a0, b0);
+        const auto step = [&](int s, auto loads) {
+          read(lds + (s & 1) * kStage, 1, a1, b1);
+          multiply(a0, b0);
+          interleave(std::integral_constant<int, 0>());
+          arrive();
+          if constexpr (decltype(loads)::value) issue(s);
+          read(lds + ((s & 1) ^ 1) * kStage, 0, a0, b0);      // (behind the last tile: something from LDS, for nothing)
+          multiply(a1, b1);
+          interleave(loads);
+        };
+        int s = 0;
+        for (; s + 2 < direct; s++) step(s, std::integral_constant<int, LA::N + LB::N>());
+        for (; s < direct; s++) step(s, std::integral_constant<int, 0>());
+      } else {
+        for (int s = 0; s < direct; s++) {
+          arrive();
+          if (s + 1 < direct) issue(s + 1);
+          frag a[MI], b[NI];
+#pragma unroll
+          for (int ks = 0; ks < 2; ks++) {
+            read(lds + (s & 1) * kStage, ks, a, b);
+            multiply(a, b);
+          }
+        }
       }
-      multiply(lds[s & 1]);
       __syncthreads();
     }
   }
   // what is left of the contraction (everything, where the operands' alignment does not allow the direct way)
-  const int from = DIRECT ? whole : 0;
-  if (from < steps) {
-    typename Loader<T, BM, A_ACROSS, THREADS>::chunk va[Loader<T, BM, A_ACROSS, THREADS>::N];
-    typename Loader<T, BN, B_ACROSS, THREADS>::chunk vb[Loader<T, BN, B_ACROSS, THREADS>::N];
-    la.fetch(first + from * BK, va);
-    lb.fetch(first + from * BK, vb);
-    la.store(lds[0], va);
-    lb.store(lds[0] + TA::kBytes, vb);
+  if (direct < steps) {
+    typename LA::chunk va[LA::N];
+    typename LB::chunk vb[LB::N];
+    la.fetch(first + direct * BK, va);
+    lb.fetch(first + direct * BK, vb);
+    la.store(lds, va);
+    lb.store(lds + TA::kBytes, vb);
     __syncthreads();
-    for (int s = from; s < steps; s++) {
-      const int now = (s - from) & 1;
+    for (int s = direct; s < steps; s++) {
+      const int now = (s - direct) & 1;
       if (s + 1 < steps) {
         la.fetch(first + (s + 1) * BK, va);
         lb.fetch(first + (s + 1) * BK, vb);
       }
-      multiply(lds[now]);
+      frag a[MI], b[NI];
+#pragma unroll
+      for (int ks = 0; ks < 2; ks++) {
+        read(lds + now * kStage, ks, a, b);
+        multiply(a, b);
+      }
       if (s + 1 < steps) {
-        la.store(lds[now ^ 1], va);
-        lb.store(lds[now ^ 1] + TA::kBytes, vb);
+        la.store(lds + (now ^ 1) * kStage, va);
+        lb.store(lds + (now ^ 1) * kStage + TA::kBytes, vb);
       }
       __syncthreads();
     }
   }
   // The epilogue goes through LDS, a part of each wavefront's rows at a time (as many as its share of the tiles' memory holds): out of the accumulators' layout (4 columns of one of 16 rows
-  // per lane) into runs of whole rows, so that what is read and written beside it are lines, and so that its code stands here once.  A row's chunk c of 4 lies at c ^ a function of the
-  // row that differs among the 16 rows that are written at once.
-  constexpr int CW = BN / WN, Q = CW / 4, HOLD = (int)sizeof(lds) / (WM * WN) / (CW * 4), PASS = HOLD < BM / WM ? HOLD / 16 * 16 : BM / WM;
-  static_assert(PASS >= 16 && (BM / WM) % PASS == 0, "rows per pass");
-  f4 *mine = (f4 *)((char *)lds + wave * ((int)sizeof(lds) / (WM * WN)));
+  // per lane) into runs of whole rows, so that what is read and written beside it are lines.  A row's chunk c of 4 lies at c ^ a function of the row that differs among the 16 rows that are
+  // written at once.
+  constexpr int CW = BN / WN, Q = CW / 4, SHARE = (int)sizeof(lds) / (WM * WN) / 16 * 16, HOLD = SHARE / (CW * 4) / 16 * 16;
+  constexpr int PASS = HOLD >= BM / WM ? BM / WM : BM / WM / 2, STRIDE = 64 / (Q / 2), U = PASS / STRIDE;      // rows per pass, rows between a lane's, and rows per lane
+  static_assert(PASS >= 16 && PASS <= HOLD && (BM / WM) % PASS == 0 && U >= 1, "rows per pass");
+  f4 *mine = (f4 *)(lds + wave * SHARE);
   const int m0 = tm * BM + wm * (BM / WM), n0 = tn * BN + wn * CW;
+  float *sums = p.partial + ((long long)(tile - p.whole) * p.parts + part) * (BM * BN) + wm * (BM / WM) * BN + wn * CW;
 #pragma unroll
   for (int i0 = 0; i0 < MI; i0 += PASS / 16) {
 #pragma unroll
@@ -255,41 +355,38 @@ __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product
         mine[r * Q + (c ^ (r / (16 / Q) & (Q - 1)))] = acc[i0 + i][j];
       }
     wave_fence();
+    const int r0 = lane / (Q / 2), c = lane % (Q / 2) * 2;      // this lane's first row and columns of the pass
+    const auto value = [&](int u) {
+      const int r = r0 + u * STRIDE, f = r / (16 / Q) & (Q - 1);
+      return __builtin_shufflevector(mine[r * Q + (c ^ f)], mine[r * Q + ((c + 1) ^ f)], 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    if (split) {
 #pragma unroll 1
-    for (int e = lane; e < PASS * Q; e += 64) {
-      const int r = e / Q, c = e % Q, col = n0 + c * 4;
-      const long long row = m0 + i0 * 16 + r;
-      if (row >= p.m || col >= p.n) continue;
-      const f4 v = mine[r * Q + (c ^ (r / (16 / Q) & (Q - 1)))];
-      if (p.e.partial) {
-        float *out = p.e.partial + ((long long)blockIdx.y * p.m + row) * p.n + col;
-        typedef float fu __attribute__((ext_vector_type(4), aligned(4)));
-        if (p.n - col >= 4) *(fu *)out = v;
-        else
-#pragma unroll
-          for (int k = 0; k < 4; k++) if (col + k < p.n) out[k] = v[k];
-      } else finish<T>(p.e, row, col, p.n, v);
-    }
+      for (int u = 0; u < U; u++) *(f8 *)(sums + (i0 * 16 + r0 + u * STRIDE) * BN + c * 4) = value(u);
+    } else if (n0 + CW <= p.n && p.e.act <= kRelu) finish_rows<T, U>(p.e, m0 + i0 * 16 + r0, STRIDE, p.m, n0 + c * 4, value);
+    else
+#pragma unroll 1
+      for (int u = 0; u < U; u++) {
+        const long long row = m0 + i0 * 16 + r0 + u * STRIDE;
+        if (row < p.m && n0 + c * 4 < p.n) finish<T>(p.e, row, n0 + c * 4, p.n - n0 - c * 4, value(u));
+      }
     wave_fence();
   }
 }
 
-// sums of the contraction's parts, in their order, and the epilogue: 4 columns per thread
-template <typename T> __global__ __launch_bounds__(256) void k3_affine_join_kernel(Epilogue e, int m, int n, int parts) {
-  const int quads = (n + 3) / 4;
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / quads;
-  const int col = (int)(id - row * quads) * 4;
-  if (row >= m) return;
-  f4 v = {};
-  for (int s = 0; s < parts; s++) {
-    const float *in = e.partial + ((long long)s * m + row) * n + col;
-    typedef float fu __attribute__((ext_vector_type(4), aligned(4)));
-    if (n - col >= 4) v += *(const fu *)in;
-    else
-#pragma unroll
-      for (int j = 0; j < 4; j++) if (col + j < n) v[j] += in[j];
-  }
-  finish<T>(e, row, col, n, v);
+// the sums of a split tile's parts, in their order, and the epilogue: 8 columns per thread
+template <typename T> __global__ __launch_bounds__(256) void k3_affine_join_kernel(Product p, int bm, int bn) {
+  const int groups = bm * bn / 2048, t = blockIdx.x / groups, e = (blockIdx.x - t * groups) * 256 + threadIdx.x, r = e / (bn / 8), c = e % (bn / 8) * 8;
+  int tm, tn;
+  place(p, p.whole + t, tm, tn);
+  const long long row = (long long)tm * bm + r;
+  const int col = tn * bn + c;
+  if (row >= p.m || col >= p.n) return;
+  const float *in = p.partial + (long long)t * p.parts * bm * bn + r * bn + c;
+  f8 v = *(const f8 *)in;
+#pragma unroll 4
+  for (int s = 1; s < p.parts; s++) v += *(const f8 *)(in + (long long)s * bm * bn);
+  finish<T>(p.e, row, col, p.n - col, v);
 }
 
 // dz = dy act'(pre), rounded to the matrices' type for the products (null: dz is dy), and the sums over a strip of rows of the unrounded values: partial [strip][cols]; a workgroup takes 64
@@ -341,34 +438,42 @@ __global__ __launch_bounds__(1024) void k3_affine_bias_join_kernel(const float *
 
 // ---- plans
 
-struct Plan { int size, tiles_m, tiles_n, parts, steps_per_part; int64_t bytes; };      // size: 0 = 32 x 64, 1 = 64 x 64, 2 = 128 x 128, 3 = 256 x 256 outputs per workgroup
-const int kTile[4][2] = {{32, 64}, {64, 64}, {128, 128}, {256, 256}};
+// A workgroup's outputs, how many workgroups the chip holds at once, and how long an LDS tile of 64 steps takes, in us: alone on its compute unit, and each of those that share one when there
+// are enough of them to keep it busy.  Measured in bf16 (one size for all of a product): 2048 x 2048 x 2048 in 50.6 / 27.7 / 27.0 / 39.2 us from the largest size to the smallest,
+// 512 x 4096 x 2048 in 49.1 / 25.7 / 15.8 / 19.2, 32 x 8192 x 1024 in 25.8 / 13.6 / 7.8 / 7.0, 42752 x 1536 x 1536 in 173 / 192 / - / -.
+struct Size { int bm, bn, slots; double alone, shared; };
+const Size kSizes[4] = {{32, 64, 1536, 0.25, 0.115}, {64, 64, 1024, 0.3, 0.19}, {128, 128, 512, 0.7, 0.5}, {256, 256, 256, 1.5, 1.7}};
+constexpr int kStep = 64;
+struct Plan { int size, tiles_m, tiles_n, whole, parts, steps_per_part; int64_t bytes; };
 
-// the largest tile whose tiles (with the contraction in parts where they are few) still cover the 256 compute units
+// The size and the parts of the last tiles that cost least by a model of rounds over the chip: rounds of whole tiles, rounds of the parts, and the parts' way through memory.
 Plan plan_product(int m, int n, int k) {
-  const int steps = (k + BK - 1) / BK;
   Plan best{};
-  for (int size = 3; size >= 0; size--) {
-    if (size > 0 && m <= kTile[size - 1][0] && size < 3) { if (m <= kTile[size - 1][0]) continue; }
-    Plan p{};
-    p.size = size;
-    p.tiles_m = (m + kTile[size][0] - 1) / kTile[size][0];
-    p.tiles_n = (n + kTile[size][1] - 1) / kTile[size][1];
-    const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    const int want = size == 3 ? 200 : 256;
-    int parts = 1;
-    if (tiles < want) parts = std::max(1, std::min<int>(steps / (size == 0 ? 2 : 4), (int)((want + tiles - 1) / tiles)));
-    p.steps_per_part = (steps + parts - 1) / parts;
-    p.parts = steps ? (steps + p.steps_per_part - 1) / p.steps_per_part : 1;
-    best = p;
-    if (tiles * p.parts >= want || size == 0) break;
+  double least = 1e300;
+  for (int size = 0; size < 4; size++) {
+    const Size &z = kSizes[size];
+    const long long tm = (m + z.bm - 1) / z.bm, tn = (n + z.bn - 1) / z.bn, tiles = tm * tn, steps = std::max(1, (k + kStep - 1) / kStep);
+    if (tiles > 1 << 28) continue;
+    const auto time = [&](long long units, long long each) {
+      const long long rounds = units / z.slots, rest = units % z.slots;
+      return (each + 2.0) * (rounds * (z.slots / 256) * z.shared + (rest ? std::max(z.alone, (double)((rest + 255) / 256) * z.shared) : 0.0));
+    };
+    for (int parts = 1; parts <= 16; parts++) {
+      const long long whole = parts == 1 ? tiles : tiles / z.slots * z.slots, rest = tiles - whole, per = (steps + parts - 1) / parts, used = (steps + per - 1) / per;
+      if (parts > 1 && (rest == 0 || used != parts || per < 2)) continue;
+      const double bytes = parts > 1 ? (double)rest * parts * z.bm * z.bn * 4 : 0.0;
+      const double us = parts == 1 ? time(tiles, steps) : time(whole, steps) + time(rest * parts, per) + 3.0 + 2.0 * bytes / 5e6;
+      if (us < least) {
+        least = us;
+        best = {size, (int)tm, (int)tn, (int)whole, parts, (int)per, (int64_t)bytes};
+      }
+    }
   }
-  best.bytes = best.parts > 1 ? (int64_t)best.parts * m * n * 4 : 0;
   return best;
 }
 
 template <typename T, bool A_ACROSS, bool B_ACROSS, bool DIRECT> void launch_product(const Plan &pl, const Product &p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.parts);
+  const dim3 grid((unsigned)(p.whole + (p.tiles_m * p.tiles_n - p.whole) * p.parts));
   switch (pl.size) {
     case 0: hipLaunchKernelGGL((k3_affine_product_kernel<T, 32, 64, 1, 4, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
     case 1: hipLaunchKernelGGL((k3_affine_product_kernel<T, 64, 64, 2, 2, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
@@ -379,14 +484,14 @@ template <typename T, bool A_ACROSS, bool B_ACROSS, bool DIRECT> void launch_pro
 template <bool ACROSS> bool direct_ok(const void *p, long long ld, int rows) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && (!ACROSS || rows % 8 == 0); }
 template <typename T, bool A_ACROSS, bool B_ACROSS> int run_product(Product p, void *workspace, hipStream_t st) {
   const Plan pl = plan_product(p.m, p.n, p.k);
-  p.tiles_m = pl.tiles_m; p.tiles_n = pl.tiles_n; p.parts = pl.parts; p.steps_per_part = pl.steps_per_part;
-  p.e.partial = pl.parts > 1 ? (float *)workspace : nullptr;
+  p.tiles_m = pl.tiles_m; p.tiles_n = pl.tiles_n; p.whole = pl.whole; p.parts = pl.parts; p.steps_per_part = pl.steps_per_part;
+  p.partial = (float *)workspace;
   if (direct_ok<A_ACROSS>(p.a, p.lda, p.m) && direct_ok<B_ACROSS>(p.b, p.ldb, p.n)) launch_product<T, A_ACROSS, B_ACROSS, true>(pl, p, st);
   else launch_product<T, A_ACROSS, B_ACROSS, false>(pl, p, st);
   K3_HIP_CHECK(hipGetLastError());
-  if (pl.parts > 1) {
-    const long long quads = (long long)p.m * ((p.n + 3) / 4);
-    hipLaunchKernelGGL((k3_affine_join_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, p.e, p.m, p.n, pl.parts);
+  if (pl.bytes) {
+    const Size &z = kSizes[pl.size];
+    hipLaunchKernelGGL((k3_affine_join_kernel<T>), dim3((unsigned)((p.tiles_m * p.tiles_n - p.whole) * (z.bm * z.bn / 2048))), dim3(256), 0, st, p, z.bm, z.bn);
     K3_HIP_CHECK(hipGetLastError());
   }
   return K3_OK;
