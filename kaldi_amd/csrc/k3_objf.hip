@@ -12,7 +12,7 @@ namespace {
 using namespace k3;
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr float kInf = __builtin_inff();
+constexpr float kInf = __builtin_inff(), kMaxFloat = 3.402823466e38f;
 constexpr int kMaxTop = 64;              // alternatives per row: one per lane of a wavefront
 constexpr int kMaxTeacher = 1024;        // teacher entries per row: their probabilities lie in LDS
 constexpr int kMaxSplits = 64;           // parts of a row: one per lane of the wavefront that joins them
@@ -154,35 +154,61 @@ __device__ inline void write_alternative(const ScoreArgs &p, long long row, int 
   if (p.alt_labels) p.alt_labels[row * p.top + rank] = fine ? col : -1;
 }
 
-// a lane's E chunks of columns [begin, end) of a row, -inf behind `end`; col = the chunks' first columns
-template <typename T, int NW, int E> __device__ inline void load_part(const T *z, int begin, int end, typename Chunk<T>::type (&v)[E], int (&col)[E]) {
-  constexpr int N = Chunk<T>::N;
-  const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
+// Columns [begin, end) of a row in the registers of NW wavefronts: chunk t + 64 NW i of them is lane t's i-th.  Which of a lane's chunks are whole is the same for all lanes but for one chunk
+// (number `whole`, the row's end lies in it), so whole chunks are loaded and stored without a branch of the lanes, from one base address.
+template <typename T, int NW, int E> struct Part {
+  static constexpr int N = Chunk<T>::N, SPAN = 64 * NW * N;      // columns of one chunk of every lane
+  int begin, end, whole, t;
+  __device__ inline Part(int begin, int end) : begin(begin), end(end), whole((end - begin) / SPAN), t(NW == 1 ? threadIdx.x & 63 : threadIdx.x) {}
+  __device__ inline int column(int e) const { return begin + e / N * SPAN + t * N + e % N; }
+  // -inf behind `end`
+  __device__ inline void load(const T *row, Packed (&v)[E]) const {
+    const Packed tail = load_packed<T>(row, begin + whole * SPAN + t * N, end - begin - whole * SPAN - t * N, (T)-kInf);
+    const int fill = sizeof(T) == 4 ? (int)0xff800000 : std::is_same<T, bf16>::value ? (int)0xff80ff80 : (int)0xfc00fc00;
 #pragma unroll
-  for (int i = 0; i < E; i++) {
-    col[i] = begin + (t + i * 64 * NW) * N;
-    const int valid = end - col[i];
-    if (valid >= N) v[i] = *reinterpret_cast<const typename Chunk<T>::type *>(z + col[i]);
-    else
-#pragma unroll
-      for (int j = 0; j < N; j++) v[i][j] = j < valid ? z[col[i] + j] : (T)-kInf;
+    for (int i = 0; i < E; i++) {
+      if (i < whole) v[i] = __builtin_bit_cast(Packed, *reinterpret_cast<const typename Chunk<T>::type *>(row + begin + i * SPAN + (unsigned)(t * N)));
+      else v[i] = i == whole ? tail : Packed{fill, fill, fill, fill};
+    }
   }
-}
-template <typename T, int E> __device__ inline float largest(const typename Chunk<T>::type (&v)[E]) {
+  // value(packed chunk, j) rounded to the row's type
+  template <typename F> __device__ inline void store(T *row, const Packed (&v)[E], F value) const {
+    Packed last = v[0];
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+      if (i < whole) {
+        typename Chunk<T>::type o;
+#pragma unroll
+        for (int j = 0; j < N; j++) o[j] = (T)value(v[i], i * N + j, j);
+        *reinterpret_cast<typename Chunk<T>::type *>(row + begin + i * SPAN + (unsigned)(t * N)) = o;
+      } else if (i == whole) last = v[i];
+    }
+    const int col = begin + whole * SPAN + t * N;
+    if (col >= end) return;
+    Packed one[1] = {last};
+    keep_packed<T, 1>(one);
+    last = one[0];
+    typename Chunk<T>::type o;
+#pragma unroll
+    for (int j = 0; j < N; j++) o[j] = (T)value(last, whole * N + j, j);
+    store_chunk(row, col, end - col, o);
+  }
+};
+template <typename T, int E> __device__ inline float largest(const Packed (&v)[E]) {
   float m = -kInf;
 #pragma unroll
   for (int i = 0; i < E; i++)
 #pragma unroll
-    for (int j = 0; j < Chunk<T>::N; j++) m = fmaxf(m, to_f32(v[i][j]));
+    for (int j = 0; j < Chunk<T>::N; j++) m = fmaxf(m, element<T>(v[i], j));
   return m;
 }
 // s of a row part whose largest value is -inf: 0, or NaN where there are NaNs beside it
-template <typename T, int NW, int E> __device__ inline float empty_sum(const typename Chunk<T>::type (&v)[E], float *sh) {
+template <typename T, int NW, int E> __device__ inline float empty_sum(const Packed (&v)[E], float *sh) {
   float bad = 0.0f;
 #pragma unroll
   for (int i = 0; i < E; i++)
 #pragma unroll
-    for (int j = 0; j < Chunk<T>::N; j++) bad = to_f32(v[i][j]) == to_f32(v[i][j]) ? bad : 1.0f;
+    for (int j = 0; j < Chunk<T>::N; j++) bad = element<T>(v[i], j) == element<T>(v[i], j) ? bad : 1.0f;
   return block_max<NW>(bad, sh) > 0.0f ? __builtin_nanf("") : 0.0f;
 }
 
@@ -191,7 +217,7 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
   constexpr int N = Chunk<T>::N, RPB = NW == 1 ? 4 : 1;
   __shared__ float sh[4 * NW];
   __shared__ TopShared<NW> top_sh[RPB];
-  const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x, sub = NW == 1 ? threadIdx.x >> 6 : 0;
+  const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x, sub = NW == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const long long item = (long long)blockIdx.x * RPB + sub;
   if (item >= (long long)p.rows * p.splits) return;      // (NW = 1: a whole wavefront, and no barrier spans wavefronts)
   const long long row = item / p.splits;
@@ -200,24 +226,26 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
   int y;
   const bool has_label = !p.partial && label_of(p, row, y);
   const float label_value = has_label ? to_f32(z[y]) : 0.0f;
-  typename Chunk<T>::type v[E];
-  int col[E];
-  load_part<T, NW, E>(z, begin, end, v, col);
+  Packed v[E];
+  const Part<T, NW, E> columns(begin, end);
+  columns.load(z, v);
   const float lane_max = largest<T, E>(v), m = block_max<NW>(lane_max, sh);
+  keep_packed<T, E>(v);
   float s = 0.0f, u = 0.0f;
 #pragma unroll
   for (int i = 0; i < E; i++)
 #pragma unroll
     for (int j = 0; j < N; j++) {
-      const float d = (to_f32(v[i][j]) - m) * p.a, e = exp2_fast(d);
+      const float d = (element<T>(v[i], j) - m) * p.a, e = exp2_fast(d);
       s += e;
       u += e * fmaxf(d, -16384.0f);      // (e = 0 where d = -inf: the product is to be 0)
     }
   block_sum2<NW>(s, u, sh + NW);
+  keep_packed<T, E>(v);
   if (m == -kInf) s = u = empty_sum<T, NW, E>(v, sh + 3 * NW);
-  const auto value = [&](int i, int j) { return to_f32(v[i][j]); };
+  const auto value = [&](int i, int j) { return element<T>(v[i], j); };
   const auto fetch = [&](int e, float &v, int &c) {
-    c = begin + (t + e / N * 64 * NW) * N + e % N;
+    c = columns.column(e);
     if (c < end) v = to_f32(z[c]);
     else { v = -kInf; c = -1; }
   };
@@ -283,30 +311,22 @@ template <typename T> __global__ __launch_bounds__(256) void k3_row_scores_join_
 template <typename T> __global__ __launch_bounds__(256) void k3_label_deriv_kernel(const T *z, long long ld, const int *labels, const float *stats, const float *entropy,
     const float *log_prob_deriv, const float *entropy_deriv, T *dz, long long ldd, int cols, int segments, long long items) {
   constexpr int N = Chunk<T>::N, E = 4;
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long item = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= items) return;
   const long long row = item / segments;
   const int begin = (int)(item - row * segments) * (64 * E * N), end = min(cols, begin + 64 * E * N);
-  typename Chunk<T>::type v[E];
-  int col[E];
-  load_part<T, 1, E>(z + row * ld, begin, end, v, col);
+  const Part<T, 1, E> columns(begin, end);
+  Packed v[E];
+  columns.load(z + row * ld, v);
   const float m = stats[2 * row], log_sum = stats[2 * row + 1], h = entropy_deriv ? entropy_deriv[row] : 0.0f;
   int y = labels ? labels[row] : -1;
   if (y < 0 || y >= cols) y = -1;
   const float g = y >= 0 && log_prob_deriv ? log_prob_deriv[row] : 0.0f, b = -h, c = -g - (h != 0.0f ? h * entropy[row] : 0.0f);
   const bool empty = m == -kInf;
-#pragma unroll
-  for (int i = 0; i < E; i++) {
-    typename Chunk<T>::type o;
-#pragma unroll
-    for (int j = 0; j < N; j++) {
-      const float lq = to_f32(v[i][j]) - m - log_sum, q = exp2_fast(lq * kLog2e);
-      float d = q * __builtin_fmaf(b, fmaxf(lq, -16384.0f), c);      // (q = 0 where lq = -inf)
-      if (col[i] + j == y) d += g;
-      o[j] = (T)(empty ? 0.0f : d);
-    }
-    store_chunk(dz + row * ldd, col[i], end - col[i], o);
-  }
+  columns.store(dz + row * ldd, v, [&](Packed w, int e, int j) {
+    const float lq = element<T>(w, j) - m - log_sum, q = exp2_fast(lq * kLog2e), d = q * __builtin_fmaf(b, fmaxf(lq, -16384.0f), c);      // (q = 0 where lq = -inf)
+    return empty ? 0.0f : columns.column(e) == y ? d + g : d;
+  });
 }
 
 struct DistillArgs {
@@ -358,53 +378,48 @@ template <int NW> __device__ inline float teacher_objf(const DistillArgs &p, con
 
 // One row per NW wavefronts, held in registers from the sums to the derivative: read once, written once.  The teacher's columns are corrected behind the row's own store (by the same
 // workgroup, after a barrier).
-template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k3_distill_kernel(DistillArgs p) {
+template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW, NW >= 8 ? 4 : 1) void k3_distill_kernel(DistillArgs p) {
   constexpr int N = Chunk<T>::N, RPB = NW == 1 ? 4 : 1;
   __shared__ float sh[6 * NW];
   extern __shared__ Entry entries[];
-  const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x, sub = NW == 1 ? threadIdx.x >> 6 : 0;
+  const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x, sub = NW == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const long long row = (long long)blockIdx.x * RPB + sub;
   if (row >= p.rows) return;      // (NW = 1: a whole wavefront, and no barrier spans wavefronts)
   Entry *entry = entries + sub * p.top;
   const float teacher_max = read_teacher<T>(p, row, entry, t, 64 * NW);
-  typename Chunk<T>::type v[E];
-  int col[E];
-  load_part<T, NW, E>((const T *)p.z + row * p.ld, 0, p.cols, v, col);
+  Packed v[E];
+  const Part<T, NW, E> columns(0, p.cols);
+  columns.load((const T *)p.z + row * p.ld, v);
+  // each lane's sum against its own largest value so far, so that chunks are worked on while later ones are still on their way
+  float lm = -kMaxFloat, s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    float c = element<T>(v[i], 0);
+#pragma unroll
+    for (int j = 1; j < N; j++) c = fmaxf(c, element<T>(v[i], j));
+    c = fmaxf(c, lm);
+    s *= exp2_fast((lm - c) * p.a);
+    lm = c;
+#pragma unroll
+    for (int j = 0; j < N; j++) s += exp2_fast((element<T>(v[i], j) - c) * p.a);
+  }
   const Teacher teacher = teacher_softmax<T, NW>(p, row, entry, teacher_max, t, sh);
-  const float m = block_max<NW>(largest<T, E>(v), sh + 2 * NW);
-  const bool empty = m == -kInf;
-  const float empty_s = empty ? empty_sum<T, NW, E>(v, sh + 5 * NW) : 0.0f;
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < E; i++)
-#pragma unroll
-    for (int j = 0; j < N; j++) {
-      const float e = exp2_fast((to_f32(v[i][j]) - m) * p.a);
-      if constexpr (sizeof(T) == 4) v[i][j] = e;      // kept in the element's place; in half precision it is computed again below
-      s += e;
-    }
-  s = block_sum<NW>(s, sh + 3 * NW);
-  if (empty) s = empty_s;
+  float m = block_max<NW>(lm, sh + 2 * NW);
+  s = block_sum<NW>(s * exp2_fast((lm - m) * p.a), sh + 3 * NW);
+  const bool empty = s == 0.0f;      // (the row's largest value adds 1: nothing but -inf)
+  if (empty) m = -kInf;
   const float w = (p.weights ? p.weights[row] : 1.0f) * p.temperature;
   const float f = teacher_objf<NW>(p, entry, teacher, m, s, t, sh + 4 * NW);
   if (t == 0) p.objf[row] = teacher.live ? w * p.temperature * f : 0.0f;
   if (!p.dz) return;
   T *dz = (T *)p.dz + row * p.ldd;
-  const bool zero = !teacher.live || (empty && s == s);
-  const float g = -w / s;
-#pragma unroll
-  for (int i = 0; i < E; i++) {
-    typename Chunk<T>::type o;
-#pragma unroll
-    for (int j = 0; j < N; j++) {
-      float e;
-      if constexpr (sizeof(T) == 4) e = v[i][j];
-      else e = exp2_fast((to_f32(v[i][j]) - m) * p.a);
-      o[j] = (T)(zero ? 0.0f : g * e);
-    }
-    store_chunk(dz, col[i], p.cols - col[i], o);
+  if (!teacher.live || empty) {
+    for (int c = t; c < p.cols; c += 64 * NW) dz[c] = (T)0.0f;
+    return;
   }
-  if (zero) return;
+  keep_packed<T, E>(v);
+  const float g = -w / s;
+  columns.store(dz, v, [&](Packed w, int, int j) { return g * exp2_fast((element<T>(w, j) - m) * p.a); });
   row_barrier<NW>();
   for (int k = t; k < p.top; k += 64 * NW) {
     const int c = entry[k].col;
@@ -440,9 +455,9 @@ template <typename T> __global__ __launch_bounds__(256) void k3_distill_deriv_ke
   T *dz = (T *)p.dz + row * p.ldd;
   const int *index = p.indexes + row * p.ld_indexes;
   const float *prob = p.prob + row * p.top;
-  typename Chunk<T>::type v[E];
-  int col[E];
-  load_part<T, 4, E>(z, begin, end, v, col);
+  Packed v[E];
+  const Part<T, 4, E> columns(begin, end);
+  columns.load(z, v);
   const float4 c = p.coef[row];
   constexpr int K = kMaxTeacher / 256;
   float zk[K];      // read before anything of this part is written: dz may be z
@@ -452,13 +467,7 @@ template <typename T> __global__ __launch_bounds__(256) void k3_distill_deriv_ke
     zk[i] = j >= begin && j < end ? to_f32(z[j]) : 0.0f;
   }
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < E; i++) {
-    typename Chunk<T>::type o;
-#pragma unroll
-    for (int j = 0; j < N; j++) o[j] = (T)(c.w == 0.0f ? 0.0f : c.y * exp2_fast((to_f32(v[i][j]) - c.x) * p.a));
-    store_chunk(dz, col[i], end - col[i], o);
-  }
+  columns.store(dz, v, [&](Packed w, int, int j) { return c.w == 0.0f ? 0.0f : c.y * exp2_fast((element<T>(w, j) - c.x) * p.a); });
   if (c.w == 0.0f) return;
   __syncthreads();
 #pragma unroll
@@ -473,22 +482,26 @@ template <typename T> __global__ __launch_bounds__(256) void k3_distill_deriv_ke
 
 // ---- shapes
 
-// wavefronts and chunks per thread that hold `cols` columns (one wavefront up to 8 chunks per lane, then 4, then `most_waves`); e = 0: too wide
+// wavefronts and chunks per thread that hold `cols` columns: one wavefront up to 8 chunks per lane, then 4 up to 8, 8 up to 16 (two such workgroups, with 64 of their 128 registers full of
+// row, fill a compute unit) and 16 up to 16; e = 0: too wide
 struct Shape { int nw, e; };
 template <typename T> Shape shape_of(int cols, int least_waves, int most_waves) {
   const int chunks = (cols + Chunk<T>::N - 1) / Chunk<T>::N;
-  for (int nw = least_waves; nw <= most_waves; nw *= 4) {
-    const int e = (chunks + 64 * nw - 1) / (64 * nw), most = nw == 16 ? 16 : 8;
-    if (e <= most) return {nw, e <= 4 ? e : e <= 6 ? 6 : e <= 8 ? 8 : e <= 12 ? 12 : 16};
+  for (const Shape hold : {Shape{1, 8}, Shape{4, 8}, Shape{8, 16}, Shape{16, 16}}) {
+    const int e = (chunks + 64 * hold.nw - 1) / (64 * hold.nw);
+    if (hold.nw >= least_waves && hold.nw <= most_waves && e <= hold.e) return {hold.nw, e <= 4 ? e : e <= 6 ? 6 : e <= 8 ? 8 : e <= 12 ? 12 : 16};
   }
   return {0, 0};
 }
 // f(NW, E) as integral constants
 template <int NW, typename F> void with_chunks(int e, F f) {
 #define K3_E(v) case v: f(std::integral_constant<int, NW>(), std::integral_constant<int, v>()); return
-  switch (e) {
-    K3_E(1); K3_E(2); K3_E(3); K3_E(4); K3_E(6); K3_E(8);
-    default: if constexpr (NW == 16) { switch (e) { K3_E(12); K3_E(16); } }
+  if constexpr (NW <= 4) {
+    switch (e) { K3_E(1); K3_E(2); K3_E(3); K3_E(4); K3_E(6); K3_E(8); default: return; }
+  } else if constexpr (NW == 8) {
+    switch (e) { K3_E(6); K3_E(8); K3_E(12); K3_E(16); default: return; }
+  } else {
+    switch (e) { K3_E(12); K3_E(16); default: return; }
   }
 #undef K3_E
 }
@@ -538,14 +551,11 @@ template <typename T> int label_logprobs(ScoreArgs p, void *workspace, hipStream
 
 // whether a distillation row goes through one workgroup: up to 4 wavefronts without a derivative (wider rows are read by several workgroups), up to 16 with it
 template <typename T> Shape distill_shape(int cols, int top, bool deriv) { return shape_of<T>(cols, top > 256 ? 4 : 1, deriv ? 16 : 4); }
-// rows that go through the three kernels together: their elements stay in the chip's last cache (256 MB) from the first reading to the second
-template <typename T> int distill_group(int rows, int cols) { return (int)std::min<long long>(rows, std::max<long long>(1, (64ll << 20) / ((long long)cols * (long long)sizeof(T)))); }
 template <typename T> int64_t distill_workspace(int rows, int cols, int top, bool deriv) {
   if (distill_shape<T>(cols, top, deriv).e) return 0;
-  const int group = deriv ? distill_group<T>(rows, cols) : rows;
   int splits, span;
-  split_rows<T>(group, cols, splits, span);
-  return up16((int64_t)group * splits * sizeof(Partial)) + (deriv ? (int64_t)group * 16 + up16((int64_t)group * top * 4) : 0);
+  split_rows<T>(rows, cols, splits, span);
+  return up16((int64_t)rows * splits * sizeof(Partial)) + (deriv ? (int64_t)rows * 16 + up16((int64_t)rows * top * 4) : 0);
 }
 template <typename T> int distill(DistillArgs p, void *workspace, hipStream_t st) {
   const Shape s = distill_shape<T>(p.cols, p.top, p.dz != nullptr);
@@ -556,39 +566,30 @@ template <typename T> int distill(DistillArgs p, void *workspace, hipStream_t st
     };
     if (s.nw == 1) with_chunks<1>(s.e, launch);
     else if (s.nw == 4) with_chunks<4>(s.e, launch);
+    else if (s.nw == 8) with_chunks<8>(s.e, launch);
     else with_chunks<16>(s.e, launch);
     K3_HIP_CHECK(hipGetLastError());
     return K3_OK;
   }
-  const int group = p.dz ? distill_group<T>(p.rows, p.cols) : p.rows;
-  for (int first = 0; first < p.rows; first += group) {
-    DistillArgs q = p;
-    q.rows = std::min(group, p.rows - first);
-    q.z = (const T *)p.z + first * p.ld;
-    q.values = (const T *)p.values + first * p.ld_values;
-    q.indexes = p.indexes + first * p.ld_indexes;
-    q.weights = p.weights ? p.weights + first : nullptr;
-    q.objf = p.objf + first;
-    q.dz = p.dz ? (T *)p.dz + first * p.ldd : nullptr;
-    ScoreArgs sc{};
-    sc.z = q.z; sc.ld = q.ld; sc.rows = q.rows; sc.cols = q.cols; sc.a = q.a;
-    split_rows<T>(group, q.cols, sc.splits, sc.span);
-    char *w = (char *)workspace;
-    sc.partial = (Partial *)w;
-    q.partial = sc.partial;
-    q.splits = sc.splits;
-    w += up16((int64_t)group * sc.splits * sizeof(Partial));
-    q.coef = (float4 *)w;
-    q.prob = (float *)(w + (int64_t)group * 16);
-    const int rc = launch_scores<T>(sc, st);
-    if (rc) return rc;
-    hipLaunchKernelGGL((k3_distill_join_kernel<T>), dim3((unsigned)q.rows), dim3(64), sizeof(Entry) * q.top, st, q);
+  ScoreArgs sc{};
+  sc.z = p.z; sc.ld = p.ld; sc.rows = p.rows; sc.cols = p.cols; sc.a = p.a;
+  split_rows<T>(p.rows, p.cols, sc.splits, sc.span);
+  char *w = (char *)workspace;
+  sc.partial = (Partial *)w;
+  p.partial = sc.partial;
+  p.splits = sc.splits;
+  w += up16((int64_t)p.rows * sc.splits * sizeof(Partial));
+  p.coef = (float4 *)w;
+  p.prob = (float *)(w + (int64_t)p.rows * 16);
+  const int segments = (p.cols + 256 * 4 * Chunk<T>::N - 1) / (256 * 4 * Chunk<T>::N);
+  K3_REQUIRE((long long)p.rows * segments < (1ll << 31), "k3_distill_objf_and_deriv: matrix too large");
+  const int rc = launch_scores<T>(sc, st);
+  if (rc) return rc;
+  hipLaunchKernelGGL((k3_distill_join_kernel<T>), dim3((unsigned)p.rows), dim3(64), sizeof(Entry) * p.top, st, p);
+  K3_HIP_CHECK(hipGetLastError());
+  if (p.dz) {
+    hipLaunchKernelGGL((k3_distill_deriv_kernel<T>), dim3((unsigned)(p.rows * segments)), dim3(256), 0, st, p, segments);
     K3_HIP_CHECK(hipGetLastError());
-    if (q.dz) {
-      const int segments = (q.cols + 256 * 4 * Chunk<T>::N - 1) / (256 * 4 * Chunk<T>::N);
-      hipLaunchKernelGGL((k3_distill_deriv_kernel<T>), dim3((unsigned)((long long)q.rows * segments)), dim3(256), 0, st, q, segments);
-      K3_HIP_CHECK(hipGetLastError());
-    }
   }
   return K3_OK;
 }

@@ -1,6 +1,7 @@
 // k3_rowops.h -- device helpers shared by the operators that work on rows of float / half / bfloat16 matrices (k3_layernorm.hip, k3_objf.hip) and by k3_affine.hip.
 #pragma once
 #include "k3_common.h"
+#include <type_traits>
 
 namespace k3 {
 
@@ -24,6 +25,38 @@ template <typename T> __device__ inline void store_chunk(T *row, int col, int va
   if (valid >= Chunk<T>::N) { *reinterpret_cast<typename Chunk<T>::type *>(row + col) = v; return; }
 #pragma unroll
   for (int j = 0; j < Chunk<T>::N; j++) if (j < valid) row[col + j] = v[j];
+}
+// A chunk as it is stored, in four registers whatever its type (a vector of halves that comes out of two branches is taken apart by the compiler, into a register per element)
+typedef int Packed __attribute__((ext_vector_type(4)));
+template <typename T> __device__ inline float element(Packed v, int j) {
+  const int w = sizeof(T) == 4 ? v[j] : v[j / 2];
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w);
+  else if constexpr (std::is_same<T, bf16>::value) return __builtin_bit_cast(float, j & 1 ? w & (int)0xffff0000 : w << 16);
+  else return (float)__builtin_bit_cast(f16, (unsigned short)(j & 1 ? (unsigned)w >> 16 : w & 0xffff));
+}
+// what is widened behind this is widened again, and not kept in float32 from before (twice the registers)
+template <typename T, int E> __device__ inline void keep_packed(Packed (&v)[E]) {
+  if constexpr (sizeof(T) == 2)
+#pragma unroll
+    for (int i = 0; i < E; i++) asm volatile("" : "+v"(v[i]));
+}
+// a chunk of a row of which `valid` elements exist, `otherwise` behind them
+template <typename T> __device__ inline Packed load_packed(const T *row, int col, int valid, T otherwise) {
+  if (valid >= Chunk<T>::N) return __builtin_bit_cast(Packed, *reinterpret_cast<const typename Chunk<T>::type *>(row + col));
+  Packed v;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = __builtin_bit_cast(int, j < valid ? row[col + j] : otherwise);
+  } else {
+    const unsigned short fill = __builtin_bit_cast(unsigned short, otherwise);
+    const unsigned short *p = reinterpret_cast<const unsigned short *>(row) + col;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const unsigned lo = 2 * j < valid ? p[2 * j] : fill, hi = 2 * j + 1 < valid ? p[2 * j + 1] : fill;
+      v[j] = (int)(lo | hi << 16);
+    }
+  }
+  return v;
 }
 // N floats from a vector (null: `otherwise`)
 template <int N> __device__ inline void load_params(const float *p, int col, int valid, float otherwise, float *out) {
