@@ -70,9 +70,15 @@ struct Epilogue {
   void *pre; long long ldp;
   int act;
 };
-// C [m x n] over k contraction steps, in tiles.  The first `whole` tiles are one workgroup's each; those behind them (what would leave most of the chip idle) are `parts` workgroups' each, of
-// steps_per_part LDS tiles of the contraction, whose float32 sums go to partial [tile][part][BM][BN] and are joined by k3_affine_join_kernel.
-struct Product { const void *a; long long lda; const void *b; long long ldb; int m, n, k; int tiles_m, tiles_n, whole, parts, steps_per_part; float *partial; Epilogue e; };
+// C [m x n] over k contraction steps, in tiles of `steps` LDS tiles of 64 of them.  The first `whole` tiles are one workgroup's each.  Those behind them (what would leave most of the chip
+// idle) are, one behind the other, cut into `units` runs of equal length, one workgroup's each: a tile that lies in one run is finished by it, of the others the float32 sums of every
+// run's piece go to partial [run + tile][BM][BN] (a number of its own for every piece) and are joined by k3_affine_join_kernel.
+struct Product {
+  const void *a; long long lda; const void *b; long long ldb; int m, n, k; int tiles_m, tiles_n, whole, units, steps; float *partial; Epilogue e;
+  __device__ inline int rest() const { return tiles_m * tiles_n - whole; }
+  __device__ inline long long run_start(int u) const { return (long long)u * ((long long)rest() * steps) / units; }
+  __device__ inline int run_of(long long at) const { return (int)(((at + 1) * units - 1) / ((long long)rest() * steps)); }      // which run a step lies in
+};
 
 typedef float f8 __attribute__((ext_vector_type(8)));
 
@@ -162,30 +168,33 @@ template <typename T, int ROWS, int BK, bool ACROSS, int THREADS> struct Loader 
   static constexpr int N = L::kChunks / THREADS;
   typedef T chunk __attribute__((ext_vector_type(8)));
   const T *base; long long ld; int row0, rows, k;      // the operand, its first row in this tile, its number of rows, and the contraction's length
-  const T *at[N];
+  int wave, lane;
+  const char *from;      // uniform: where the next tile's offsets count from
+  unsigned offset[N];
   __device__ inline void start(int k0) {
+    from = (const char *)(base + (ACROSS ? (long long)k0 * ld : (long long)row0 * ld + k0));
 #pragma unroll
     for (int i = 0; i < N; i++) {
       int major, c;
-      L::source((threadIdx.x / 64 * N + i) * 64 + (threadIdx.x & 63), major, c);
-      if (ACROSS) at[i] = base + (long long)(k0 + major) * ld + (row0 + c * 8 < rows ? row0 + c * 8 : 0);
-      else at[i] = base + (long long)min(row0 + major, rows - 1) * ld + k0 + c * 8;
+      L::source((wave * N + i) * 64 + lane, major, c);
+      if (ACROSS) offset[i] = 2u * (unsigned)(major * (int)ld + (row0 + c * 8 < rows ? row0 + c * 8 : 0));
+      else offset[i] = 2u * (unsigned)(min(major, rows - 1 - row0) * (int)ld + c * 8);
     }
   }
   __device__ inline void direct(unsigned lds) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const unsigned to = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x / 64 * N + i) * L::kBlock);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)at[i], (__attribute__((address_space(3))) void *)(unsigned long long)to, 16, 0, 0);
-      at[i] += ACROSS ? BK * ld : BK;
+      const unsigned to = lds + (wave * N + i) * L::kBlock;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from + offset[i]), (__attribute__((address_space(3))) void *)(unsigned long long)to, 16, 0, 0);
     }
+    from += ACROSS ? 2 * BK * ld : 2 * BK;
   }
   __device__ inline void fetch(int k0, chunk (&v)[N]) const {
     typedef T u8 __attribute__((ext_vector_type(8), aligned(2)));
 #pragma unroll
     for (int i = 0; i < N; i++) {
       int major, c;
-      L::source((threadIdx.x / 64 * N + i) * 64 + (threadIdx.x & 63), major, c);
+      L::source((wave * N + i) * 64 + lane, major, c);
       const int row = ACROSS ? k0 + major : row0 + major, col = ACROSS ? row0 + c * 8 : k0 + c * 8, last = ACROSS ? rows : k;
       const T *p = base + (long long)row * ld + col;
       if (row < (ACROSS ? k : rows) && col + 8 <= last) v[i] = *(const u8 *)p;
@@ -194,9 +203,9 @@ template <typename T, int ROWS, int BK, bool ACROSS, int THREADS> struct Loader 
         for (int j = 0; j < 8; j++) v[i][j] = row < (ACROSS ? k : rows) && col + j < last ? p[j] : (T)0.0f;
     }
   }
-  static __device__ inline void store(char *tile, const chunk (&v)[N]) {
+  __device__ inline void store(char *tile, const chunk (&v)[N]) const {
 #pragma unroll
-    for (int i = 0; i < N; i++) *(chunk *)(tile + (threadIdx.x / 64 * N + i) * L::kBlock + (threadIdx.x & 63) * 16) = v[i];
+    for (int i = 0; i < N; i++) *(chunk *)(tile + (wave * N + i) * L::kBlock + lane * 16) = v[i];
   }
 };
 
@@ -223,18 +232,25 @@ __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product
   using LB = Loader<T, BN, BK, B_ACROSS, THREADS>;
   constexpr int kStage = TA::kBytes + TB::kBytes;
   __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
-  // workgroups go round the 8 XCDs: each XCD takes a run of neighbouring tiles, which share operands in its L2; so do the parts of the last tiles
+  // workgroups go round the 8 XCDs: each XCD takes neighbouring tiles, which share operands in its L2; so do the runs of the last tiles
   const bool split = (int)blockIdx.x >= p.whole;
-  const int units = split ? (p.tiles_m * p.tiles_n - p.whole) * p.parts : p.whole, u = split ? blockIdx.x - p.whole : blockIdx.x;
-  const int per = units / 8, extra = units % 8, x = u % 8, unit = x * per + min(x, extra) + u / 8;
-  const int tile = split ? p.whole + unit / p.parts : unit, part = split ? unit % p.parts : 0;
+  const int count = split ? p.units : p.whole, u = split ? blockIdx.x - p.whole : blockIdx.x;
+  const int per = count / 8, extra = count % 8, x = u % 8, unit = x * per + min(x, extra) + u / 8;
+  const long long run_end = split ? p.run_start(unit + 1) : 0;
+  long long at = split ? p.run_start(unit) : 0;
+  do {      // one round per piece of a tile: this workgroup's tile, or what its run has of one
+  const int t = split ? (int)(at / p.steps) : 0, step0 = split ? (int)(at - (long long)t * p.steps) : 0, step1 = split ? (int)min((long long)p.steps, step0 + run_end - at) : p.steps;
+  const bool piece = step0 > 0 || step1 < p.steps;
+  at += step1 - step0;
+  int thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));      // (what is made of it is made anew for every piece, and takes no registers from the loop below)
+  const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), wm = wave / WN, wn = wave % WN;
   int tm, tn;
-  place(p, tile, tm, tn);
-  const int first = split ? part * p.steps_per_part * BK : 0, end = split ? min(p.k, first + p.steps_per_part * BK) : p.k;
-  const int direct = DIRECT ? max(end - first, 0) / BK : 0, steps = (max(end - first, 0) + BK - 1) / BK;
-  LA la{(const T *)p.a, p.lda, tm * BM, p.m, p.k};
-  LB lb{(const T *)p.b, p.ldb, tn * BN, p.n, p.k};
+  place(p, split ? p.whole + t : unit, tm, tn);
+  const int first = step0 * BK, end = min(p.k, step1 * BK);
+  const int direct = DIRECT ? (end - first) / BK : 0, steps = (end - first + BK - 1) / BK;
+  LA la{(const T *)p.a, p.lda, tm * BM, p.m, p.k, wave, lane};
+  LB lb{(const T *)p.b, p.ldb, tn * BN, p.n, p.k, wave, lane};
   f4 acc[MI][NI] = {};
   typedef typename Half<T>::frag frag;
   const auto read = [&](const char *ta, int ks, frag (&a)[MI], frag (&b)[NI]) {
@@ -344,7 +360,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product
   static_assert(PASS >= 16 && PASS <= HOLD && (BM / WM) % PASS == 0 && U >= 1, "rows per pass");
   f4 *mine = (f4 *)(lds + wave * SHARE);
   const int m0 = tm * BM + wm * (BM / WM), n0 = tn * BN + wn * CW;
-  float *sums = p.partial + ((long long)(tile - p.whole) * p.parts + part) * (BM * BN) + wm * (BM / WM) * BN + wn * CW;
+  float *sums = p.partial + (long long)(unit + t) * (BM * BN) + wm * (BM / WM) * BN + wn * CW;
 #pragma unroll
   for (int i0 = 0; i0 < MI; i0 += PASS / 16) {
 #pragma unroll
@@ -360,7 +376,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product
       const int r = r0 + u * STRIDE, f = r / (16 / Q) & (Q - 1);
       return __builtin_shufflevector(mine[r * Q + (c ^ f)], mine[r * Q + ((c + 1) ^ f)], 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    if (split) {
+    if (piece) {
 #pragma unroll 1
       for (int u = 0; u < U; u++) *(f8 *)(sums + (i0 * 16 + r0 + u * STRIDE) * BN + c * 4) = value(u);
     } else if (n0 + CW <= p.n && p.e.act <= kRelu) finish_rows<T, U>(p.e, m0 + i0 * 16 + r0, STRIDE, p.m, n0 + c * 4, value);
@@ -372,20 +388,24 @@ __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product
       }
     wave_fence();
   }
+  if (split) __syncthreads();      // (LDS is the next piece's)
+  } while (at < run_end);
 }
 
-// the sums of a split tile's parts, in their order, and the epilogue: 8 columns per thread
+// the sums of a cut tile's pieces, in their order, and the epilogue: 8 columns per thread
 template <typename T> __global__ __launch_bounds__(256) void k3_affine_join_kernel(Product p, int bm, int bn) {
   const int groups = bm * bn / 2048, t = blockIdx.x / groups, e = (blockIdx.x - t * groups) * 256 + threadIdx.x, r = e / (bn / 8), c = e % (bn / 8) * 8;
+  const int first = p.run_of((long long)t * p.steps), last = p.run_of((long long)(t + 1) * p.steps - 1);
+  if (first == last) return;      // in one run, which has finished it
   int tm, tn;
   place(p, p.whole + t, tm, tn);
   const long long row = (long long)tm * bm + r;
   const int col = tn * bn + c;
   if (row >= p.m || col >= p.n) return;
-  const float *in = p.partial + (long long)t * p.parts * bm * bn + r * bn + c;
+  const float *in = p.partial + (long long)(first + t) * bm * bn + r * bn + c;
   f8 v = *(const f8 *)in;
 #pragma unroll 4
-  for (int s = 1; s < p.parts; s++) v += *(const f8 *)(in + (long long)s * bm * bn);
+  for (int u = 1; u <= last - first; u++) v += *(const f8 *)(in + (long long)u * bm * bn);
   finish<T>(p.e, row, col, p.n - col, v);
 }
 
@@ -444,9 +464,11 @@ __global__ __launch_bounds__(1024) void k3_affine_bias_join_kernel(const float *
 struct Size { int bm, bn, slots; double alone, shared; };
 const Size kSizes[4] = {{32, 64, 1536, 0.25, 0.115}, {64, 64, 1024, 0.3, 0.19}, {128, 128, 512, 0.7, 0.5}, {256, 256, 256, 1.5, 1.7}};
 constexpr int kStep = 64;
-struct Plan { int size, tiles_m, tiles_n, whole, parts, steps_per_part; int64_t bytes; };
+struct Plan { int size, tiles_m, tiles_n, whole, units, steps; int64_t bytes; };
 
-// The size and the parts of the last tiles that cost least by a model of rounds over the chip: rounds of whole tiles, rounds of the parts, and the parts' way through memory.
+// The size and the runs of the last tiles that cost least by a model of rounds over the chip: rounds of whole tiles, the runs, and their pieces' way through memory.  The runs are a whole
+// number per tile: 256 equal runs over 72 tiles of 400 steps keep every unit busy, but no two of them are then at the same step and share an operand, and a weight derivative of
+// 6024 x 768 over 25600 rows took 346 us against 293 in 3 runs per tile.
 Plan plan_product(int m, int n, int k) {
   Plan best{};
   double least = 1e300;
@@ -454,26 +476,29 @@ Plan plan_product(int m, int n, int k) {
     const Size &z = kSizes[size];
     const long long tm = (m + z.bm - 1) / z.bm, tn = (n + z.bn - 1) / z.bn, tiles = tm * tn, steps = std::max(1, (k + kStep - 1) / kStep);
     if (tiles > 1 << 28) continue;
-    const auto time = [&](long long units, long long each) {
-      const long long rounds = units / z.slots, rest = units % z.slots;
-      return (each + 2.0) * (rounds * (z.slots / 256) * z.shared + (rest ? std::max(z.alone, (double)((rest + 255) / 256) * z.shared) : 0.0));
-    };
-    for (int parts = 1; parts <= 16; parts++) {
-      const long long whole = parts == 1 ? tiles : tiles / z.slots * z.slots, rest = tiles - whole, per = (steps + parts - 1) / parts, used = (steps + per - 1) / per;
-      if (parts > 1 && (rest == 0 || used != parts || per < 2)) continue;
-      const double bytes = parts > 1 ? (double)rest * parts * z.bm * z.bn * 4 : 0.0;
-      const double us = parts == 1 ? time(tiles, steps) : time(whole, steps) + time(rest * parts, per) + 3.0 + 2.0 * bytes / 5e6;
+    const auto round = [&](long long units, double each) { return (each + 2.0) * std::max(z.alone, (double)((units + 255) / 256) * z.shared); };
+    const auto rounds = [&](long long units, double each) { return (units / z.slots) * round(z.slots, each) + (units % z.slots ? round(units % z.slots, each) : 0.0); };
+    const auto consider = [&](long long whole, long long units, double us) {
       if (us < least) {
         least = us;
-        best = {size, (int)tm, (int)tn, (int)whole, parts, (int)per, (int64_t)bytes};
+        const long long pieces = units ? units + tiles - whole : 0;
+        best = {size, (int)tm, (int)tn, (int)whole, (int)units, (int)steps, (int64_t)pieces * z.bm * z.bn * 4};
       }
+    };
+    consider(tiles, 0, rounds(tiles, steps));
+    const long long whole = tiles / z.slots * z.slots, rest = tiles - whole;
+    if (rest == 0) continue;
+    for (int parts = 2; parts <= 16 && rest * parts <= 2 * z.slots && steps >= 2 * parts; parts++) {      // (a whole number of runs per tile)
+      const long long units = rest * parts;
+      const double bytes = (double)units * z.bm * z.bn * 4, each = (double)steps / parts;
+      consider(whole, units, rounds(whole, steps) + rounds(units, each) + 3.0 + 2.0 * bytes / 5e6);
     }
   }
   return best;
 }
 
 template <typename T, bool A_ACROSS, bool B_ACROSS, bool DIRECT> void launch_product(const Plan &pl, const Product &p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.whole + (p.tiles_m * p.tiles_n - p.whole) * p.parts));
+  const dim3 grid((unsigned)(p.whole + p.units));
   switch (pl.size) {
     case 0: hipLaunchKernelGGL((k3_affine_product_kernel<T, 32, 64, 1, 4, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
     case 1: hipLaunchKernelGGL((k3_affine_product_kernel<T, 64, 64, 2, 2, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
@@ -481,10 +506,11 @@ template <typename T, bool A_ACROSS, bool B_ACROSS, bool DIRECT> void launch_pro
     default: hipLaunchKernelGGL((k3_affine_product_kernel<T, 256, 256, 2, 4, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(512), 0, st, p); return;
   }
 }
-template <bool ACROSS> bool direct_ok(const void *p, long long ld, int rows) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && (!ACROSS || rows % 8 == 0); }
+// 16-byte aligned rows, whole chunks, and offsets within a tile that fit 32 bits
+template <bool ACROSS> bool direct_ok(const void *p, long long ld, int rows) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld <= 1 << 22 && (!ACROSS || rows % 8 == 0); }
 template <typename T, bool A_ACROSS, bool B_ACROSS> int run_product(Product p, void *workspace, hipStream_t st) {
   const Plan pl = plan_product(p.m, p.n, p.k);
-  p.tiles_m = pl.tiles_m; p.tiles_n = pl.tiles_n; p.whole = pl.whole; p.parts = pl.parts; p.steps_per_part = pl.steps_per_part;
+  p.tiles_m = pl.tiles_m; p.tiles_n = pl.tiles_n; p.whole = pl.whole; p.units = pl.units; p.steps = pl.steps;
   p.partial = (float *)workspace;
   if (direct_ok<A_ACROSS>(p.a, p.lda, p.m) && direct_ok<B_ACROSS>(p.b, p.ldb, p.n)) launch_product<T, A_ACROSS, B_ACROSS, true>(pl, p, st);
   else launch_product<T, A_ACROSS, B_ACROSS, false>(pl, p, st);
