@@ -82,6 +82,22 @@ struct Product {
 
 typedef float f8 __attribute__((ext_vector_type(8)));
 
+// (the choice of the activation outside the loop over the elements: short calls are over before much code has been fetched)
+template <int ACT> __device__ inline void activate_as(f8 &v) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) v[j] = activation(ACT, v[j]);
+}
+__device__ inline void activate(int act, f8 &v) {
+  switch (act) {
+    case kRelu: activate_as<kRelu>(v); return;
+    case kSigmoid: activate_as<kSigmoid>(v); return;
+    case kTanh: activate_as<kTanh>(v); return;
+    case kSwish: activate_as<kSwish>(v); return;
+    case kGelu: activate_as<kGelu>(v); return;
+    default: return;
+  }
+}
+
 // 8 consecutive outputs of a row, `valid` of which exist
 template <typename T> __device__ inline void finish(const Epilogue &e, long long row, int col, int valid, f8 v) {
   typedef typename Chunk<T>::type t8;
@@ -94,8 +110,7 @@ template <typename T> __device__ inline void finish(const Epilogue &e, long long
     for (int j = 0; j < 8; j++) v[j] += b[j];
   }
   if (e.pre) store_chunk((T *)e.pre + row * e.ldp, col, valid, __builtin_convertvector(v, t8));
-#pragma unroll
-  for (int j = 0; j < 8; j++) v[j] = activation(e.act, v[j]);
+  activate(e.act, v);
   if (e.residual) v += __builtin_convertvector(res, f8);
   store_chunk((T *)e.c + row * e.ldc, col, valid, __builtin_convertvector(v, t8));
 }
@@ -209,8 +224,9 @@ template <typename T, int ROWS, int BK, bool ACROSS, int THREADS> struct Loader 
   }
 };
 
-// a barrier behind which the LDS loads that the workgroup's wavefronts issued are there and their LDS reads are done (raw, so that nothing else is waited for); no memory operation crosses it
-__device__ inline void arrive() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// a barrier behind which the LDS loads that the workgroup's wavefronts issued are there, but for each one's last LEFT, and their LDS reads are done (raw, so that nothing else is waited
+// for); no memory operation crosses it
+template <int LEFT> __device__ inline void arrive() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory"); }
 
 // tiles in panels of 8 columns of them, row after row within a panel: any 32 neighbours (what an XCD works on at once) share few rows and columns of the operands
 __device__ inline void place(const Product &p, int tile, int &tm, int &tn) {
@@ -222,16 +238,17 @@ __device__ inline void place(const Product &p, int tile, int &tm, int &tn) {
 // BM x BN outputs per workgroup of WM x WN wavefronts, over LDS tiles of 64 contraction steps, two of them: one is loaded while the other is multiplied.  PIPED (the size of which a compute
 // unit holds one workgroup): a tile is two halves of 32 steps for the matrix instructions, and the fragments of a half are read from LDS among the instructions of the half before it, those of the next tile's first half too: the one barrier per
 // tile stands between the halves, where every wavefront has read all of this tile (which the loads issued behind the barrier then overwrite) and the next one has arrived.
-template <typename T, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, bool DIRECT>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_ACROSS, bool B_ACROSS, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product p) {
   constexpr int THREADS = 64 * WM * WN, MI = BM / WM / 16, NI = BN / WN / 16, BK = 64;
   constexpr bool PIPED = BM == 256;
+  static_assert(!PIPED || STAGES == 2, "the order of a piped tile is that of two");
   using TA = Tile<BM, BK, A_ACROSS>;
   using TB = Tile<BN, BK, B_ACROSS>;
   using LA = Loader<T, BM, BK, A_ACROSS, THREADS>;
   using LB = Loader<T, BN, BK, B_ACROSS, THREADS>;
   constexpr int kStage = TA::kBytes + TB::kBytes;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+  __shared__ __attribute__((aligned(1024))) char lds[STAGES * kStage];
   // workgroups go round the 8 XCDs: each XCD takes neighbouring tiles, which share operands in its L2; so do the runs of the last tiles
   const bool split = (int)blockIdx.x >= p.whole;
   const int count = split ? p.units : p.whole, u = split ? blockIdx.x - p.whole : blockIdx.x;
@@ -286,9 +303,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product
       const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char *)lds;
       la.start(first);
       lb.start(first);
-      const auto issue = [&](int s) {
-        la.direct(lds0 + (s & 1) * kStage);
-        lb.direct(lds0 + (s & 1) * kStage + TA::kBytes);
+      unsigned load = 0;      // where the next tile goes
+      const auto issue = [&](int) {
+        la.direct(lds0 + load);
+        lb.direct(lds0 + load + TA::kBytes);
+        load = load == (STAGES - 1) * kStage ? 0 : load + kStage;
       };
       issue(0);
       if constexpr (PIPED) {
@@ -300,7 +319,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product
           read(lds + (s & 1) * kStage, 1, a1, b1);
           multiply(a0, b0);
           interleave(std::integral_constant<int, 0>());
-          arrive();
+          arrive<0>();
           if constexpr (decltype(loads)::value) issue(s);
           read(lds + ((s & 1) ^ 1) * kStage, 0, a0, b0);      // (behind the last tile: something from LDS, for nothing)
           multiply(a1, b1);
@@ -310,15 +329,21 @@ __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product
         for (; s + 2 < direct; s++) step(s, std::integral_constant<int, LA::N + LB::N>());
         for (; s < direct; s++) step(s, std::integral_constant<int, 0>());
       } else {
+        // STAGES - 1 tiles are on their way while one is multiplied
+#pragma unroll
+        for (int i = 1; i < STAGES - 1; i++) if (i < direct) issue(i);
+        unsigned now = 0;
         for (int s = 0; s < direct; s++) {
-          arrive();
-          if (s + 1 < direct) issue(s + 1);
+          if (s + STAGES - 2 < direct) arrive<(STAGES - 2) * (LA::N + LB::N)>();
+          else arrive<0>();
+          if (s + STAGES - 1 < direct) issue(s + STAGES - 1);
           frag a[MI], b[NI];
 #pragma unroll
           for (int ks = 0; ks < 2; ks++) {
-            read(lds + (s & 1) * kStage, ks, a, b);
+            read(lds + now, ks, a, b);
             multiply(a, b);
           }
+          now = now == (STAGES - 1) * kStage ? 0 : now + kStage;
         }
       }
       __syncthreads();
@@ -409,35 +434,61 @@ template <typename T> __global__ __launch_bounds__(256) void k3_affine_join_kern
   finish<T>(p.e, row, col, p.n - col, v);
 }
 
-// dz = dy act'(pre), rounded to the matrices' type for the products (null: dz is dy), and the sums over a strip of rows of the unrounded values: partial [strip][cols]; a workgroup takes 64
-// chunks of 8 columns by one strip, each of its 4 wavefronts every 4th row
-template <typename T> __global__ __launch_bounds__(256) void k3_affine_slope_kernel(int act, const T *dy, long long lddy, const T *pre, long long ldp, T *dz, long long lddz, float *partial,
+template <int ACT, typename T> __device__ inline void slopes_of(Packed z, float (&d)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) d[j] = slope(ACT, element<T>(z, j));
+}
+template <typename T> __device__ inline void slopes(int act, Packed z, float (&d)[8]) {
+  switch (act) {
+    case kRelu: slopes_of<kRelu, T>(z, d); return;
+    case kSigmoid: slopes_of<kSigmoid, T>(z, d); return;
+    case kTanh: slopes_of<kTanh, T>(z, d); return;
+    case kSwish: slopes_of<kSwish, T>(z, d); return;
+    case kGelu: slopes_of<kGelu, T>(z, d); return;
+    default: return;
+  }
+}
+// dz = dy act'(pre), rounded to the matrices' type for the products (null: dz is dy), and the sums over a strip of rows of the unrounded values: sums [strip][cols]; a workgroup takes 64
+// chunks of 8 columns by one strip, each of its 4 wavefronts every 4th row, the next one on its way while this one is worked on.  (Small code counts: short calls are over before much of it has
+// been fetched.  4 rows at a time, with their activations written out, took 12.8 us on 208 rows of 173 columns.)
+template <typename T> __global__ __launch_bounds__(256) void k3_affine_slope_kernel(int act, const T *dy, long long lddy, const T *pre, long long ldp, T *dz, long long lddz, float *sums,
                                                                                      int rows, int cols, int strip) {
   __shared__ float sh[3][64][8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = (blockIdx.x * 64 + lane) * 8, valid = cols - col;
   const int r0 = blockIdx.y * strip, r1 = min(rows, r0 + strip);
   float s[8] = {};
-  if (valid > 0)
+  if (valid > 0) {
+    Packed g, z = {}, ng = {}, nz = {};
+    const auto load = [&](long long row) {
+      ng = load_packed<T>(dy + row * lddy, col, valid, (T)0.0f);
+      if (act != kNone) nz = load_packed<T>(pre + row * ldp, col, valid, (T)0.0f);
+    };
+    if (r0 + wave < r1) load(r0 + wave);
+#pragma unroll 1
     for (int row = r0 + wave; row < r1; row += 4) {
-      const typename Chunk<T>::type g = load_chunk(dy + row * lddy, col, valid);
-      typename Chunk<T>::type z = {}, o;
-      if (act != kNone) z = load_chunk(pre + row * ldp, col, valid);
+      g = ng;
+      z = nz;
+      if (row + 4 < r1) load(row + 4);
+      float d[8];
+      slopes<T>(act, z, d);
+      typename Chunk<T>::type o;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const float d = act == kNone ? to_f32(g[j]) : to_f32(g[j]) * slope(act, to_f32(z[j]));
-        s[j] += d;
-        o[j] = (T)d;
+        d[j] = act == kNone ? element<T>(g, j) : element<T>(g, j) * d[j];
+        s[j] += d[j];
+        o[j] = (T)d[j];
       }
-      if (dz) store_chunk(dz + row * lddz, col, valid, o);
+      if (dz) store_chunk(dz + (long long)row * lddz, col, valid, o);
     }
-  if (!partial) return;
+  }
+  if (!sums) return;
   if (wave)
 #pragma unroll
     for (int j = 0; j < 8; j++) sh[wave - 1][lane][j] = s[j];
   __syncthreads();
   if (wave == 0)
 #pragma unroll
-    for (int j = 0; j < 8; j++) if (j < valid) partial[(long long)blockIdx.y * cols + col + j] = ((s[j] + sh[0][lane][j]) + sh[1][lane][j]) + sh[2][lane][j];
+    for (int j = 0; j < 8; j++) if (j < valid) sums[(long long)blockIdx.y * cols + col + j] = ((s[j] + sh[0][lane][j]) + sh[1][lane][j]) + sh[2][lane][j];
 }
 __global__ __launch_bounds__(1024) void k3_affine_bias_join_kernel(const float *partial, int strips, int cols, float *db) {
   __shared__ float sh[16][64];
@@ -500,10 +551,10 @@ Plan plan_product(int m, int n, int k) {
 template <typename T, bool A_ACROSS, bool B_ACROSS, bool DIRECT> void launch_product(const Plan &pl, const Product &p, hipStream_t st) {
   const dim3 grid((unsigned)(p.whole + p.units));
   switch (pl.size) {
-    case 0: hipLaunchKernelGGL((k3_affine_product_kernel<T, 32, 64, 1, 4, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
-    case 1: hipLaunchKernelGGL((k3_affine_product_kernel<T, 64, 64, 2, 2, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
-    case 2: hipLaunchKernelGGL((k3_affine_product_kernel<T, 128, 128, 2, 2, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
-    default: hipLaunchKernelGGL((k3_affine_product_kernel<T, 256, 256, 2, 4, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(512), 0, st, p); return;
+    case 0: hipLaunchKernelGGL((k3_affine_product_kernel<T, 32, 64, 1, 4, 4, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
+    case 1: hipLaunchKernelGGL((k3_affine_product_kernel<T, 64, 64, 2, 2, 3, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
+    case 2: hipLaunchKernelGGL((k3_affine_product_kernel<T, 128, 128, 2, 2, 2, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
+    default: hipLaunchKernelGGL((k3_affine_product_kernel<T, 256, 256, 2, 4, 2, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(512), 0, st, p); return;
   }
 }
 // 16-byte aligned rows, whole chunks, and offsets within a tile that fit 32 bits
@@ -544,13 +595,15 @@ template <typename T> int affine_backward(const Backward &q, char *workspace, hi
       rest += up256((int64_t)q.rows * lddz * 2);
     }
     if (q.db) { partial = (float *)rest; rest += up256((int64_t)kMaxStrips * q.cols * 4); }
-    const int strip = std::max(16, (q.rows + kMaxStrips - 1) / kMaxStrips), strips = (q.rows + strip - 1) / strip;
+    // enough strips to fill the chip, of a row per wavefront at least; a single one writes the sums at their place
+    const int across = (q.cols + 511) / 512, least = (q.rows + kMaxStrips - 1) / kMaxStrips;
+    const int strip = std::max({4, least, (int)((long long)q.rows * across / 2048)}), strips = (q.rows + strip - 1) / strip;
     if (q.rows) {
-      hipLaunchKernelGGL((k3_affine_slope_kernel<T>), dim3((q.cols + 511) / 512, strips), dim3(256), 0, st, q.act, (const T *)q.dy, q.lddy, (const T *)q.pre, q.ldp, out, lddz, partial,
-                         q.rows, q.cols, strip);
+      hipLaunchKernelGGL((k3_affine_slope_kernel<T>), dim3(across, strips), dim3(256), 0, st, q.act, (const T *)q.dy, q.lddy, (const T *)q.pre, q.ldp, out, lddz,
+                         q.db && strips == 1 ? q.db : partial, q.rows, q.cols, strip);
       K3_HIP_CHECK(hipGetLastError());
     }
-    if (q.db) {
+    if (q.db && strips != 1) {
       hipLaunchKernelGGL(k3_affine_bias_join_kernel, dim3((q.cols + 63) / 64), dim3(1024), 0, st, partial, strips, q.cols, q.db);
       K3_HIP_CHECK(hipGetLastError());
     }

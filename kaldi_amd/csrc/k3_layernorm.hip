@@ -168,8 +168,14 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
 #pragma unroll
       for (int i = 0; i < E; i++) {
         const int col = (t + i * 64 * NW) * N;
+        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+        if (col + N <= cols)
 #pragma unroll
-        for (int j = 0; j < N; j++) if (col + j < cols) out[col + j] = which ? db[i][j] : ds[i][j];
+          for (int j = 0; j < N; j += 4)
+            *(f4 *)(out + col + j) = which ? f4{db[i][j], db[i][j + 1], db[i][j + 2], db[i][j + 3]} : f4{ds[i][j], ds[i][j + 1], ds[i][j + 2], ds[i][j + 3]};
+        else
+#pragma unroll
+          for (int j = 0; j < N; j++) if (col + j < cols) out[col + j] = which ? db[i][j] : ds[i][j];
       }
   }
 }

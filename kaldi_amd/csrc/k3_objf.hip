@@ -31,12 +31,21 @@ __device__ inline float key_value(unsigned k) { return __builtin_bit_cast(float,
 __device__ inline unsigned long long pair_key(float v, int col) { return ((unsigned long long)order_key(v) << 32) | (unsigned)~col; }
 constexpr unsigned kLowest = 0x007fffffu;      // order_key(-inf)
 
-// the largest t found by descending its bits such that at least k of the 64 lanes' keys are >= t; stops as soon as exactly k are
-__device__ inline unsigned wave_kth(unsigned key, int k) {
-  unsigned t = 0;
-  for (int bit = 31; bit >= 0; bit--) {
+// the largest t found by descending its bits, from the first one in which the keys differ, such that at least k of 64 NW keys (NW of them in each lane of a wavefront) are >= t; stops as soon
+// as exactly k are
+template <int NW> __device__ inline unsigned kth_key(const unsigned (&key)[NW], int k) {
+  float most = key_value(key[0]), least = most;
+#pragma unroll
+  for (int w = 1; w < NW; w++) { most = fmaxf(most, key_value(key[w])); least = fminf(least, key_value(key[w])); }
+  const unsigned high = order_key(wave_max(most)), differ = high ^ order_key(-wave_max(-least));
+  if (differ == 0) return high;
+  const int top = 31 - __builtin_clz(differ);
+  unsigned t = (high >> top >> 1) << top << 1;      // (the bits that all keys share)
+  for (int bit = top; bit >= 0; bit--) {
     const unsigned u = t | (1u << bit);
-    const int n = __popcll(__ballot(key >= u));
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < NW; w++) n += __popcll(__ballot(key[w] >= u));
     if (n >= k) { t = u; if (n == k) break; }
   }
   return max(t, kLowest);
@@ -56,25 +65,36 @@ template <int NW> __device__ inline void row_barrier() {
   else { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 }
 
-template <int NW> struct TopShared { unsigned long long cand[kCandidates]; unsigned long long best[NW]; unsigned tau[NW]; int count; };
+template <int NW> struct TopShared { unsigned long long cand[kCandidates + 8]; unsigned long long best[NW]; unsigned key[NW > 1 ? 64 * NW : 1], tau; int count; };
 
 // The `top` largest of the E * N <= 64 (value, column) pairs of each of 64 NW threads, handed to emit(rank, value, column) with ranks 0 .. top - 1 (value -inf and column -1 where NaNs
-// or a short row leave fewer).  value(i, j): the value a thread holds; fetch(e, v, c): the same for e = i N + j, read from memory again, with its column (-1: none); lane_max: the
-// thread's largest value (-inf: none).
-// Every lane's largest element bounds what can be among the best: with t = the top-th largest of the lanes' maxima of some wavefront, `top` elements are >= t, so only elements >= t
-// (as a rule a few times `top`) are gathered and ranked by counting.  Where more than fit are >= t (many equal values), the best are taken one after another instead.
-template <int NW, int E, int N, typename V, typename G, typename F>
-__device__ inline void emit_top(V value, G fetch, float lane_max, int top, TopShared<NW> &sh, F emit) {
+// or a short row leave fewer).  value(i, j): the value a thread holds; pick(e): the same for e = i N + j; fetch(e, v, c): the same read from memory again, with its column (-1: none);
+// column(e): its column alone; lane_max: the thread's largest value (-inf: none).
+// Every lane's largest element bounds what can be among the best: with t = the top-th largest of the lanes' maxima, `top` elements are >= t, so only elements >= t (as a rule a few more
+// than `top`) are gathered and ranked by counting.  Where more than fit are >= t (many equal values), the best are taken one after another instead.
+template <int NW, int E, int N, typename V, typename P, typename C, typename G, typename F>
+__device__ inline void emit_top(V value, P pick, C column, G fetch, float lane_max, int top, TopShared<NW> &sh, F emit) {
   constexpr int TPR = 64 * NW;
   const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
-  unsigned tau = wave_kth(order_key(lane_max), top);
+  unsigned tau;
   if (t == 0) sh.count = 0;
-  if constexpr (NW > 1) {
-    if ((threadIdx.x & 63) == 0) sh.tau[threadIdx.x >> 6] = tau;
+  if constexpr (NW > 1) {      // (one wavefront looks for t; its bits are not worth the others' time)
+    sh.key[t] = order_key(lane_max);
     __syncthreads();
+    if (t < 64) {
+      unsigned keys[NW];
 #pragma unroll
-    for (int w = 0; w < NW; w++) tau = max(tau, sh.tau[w]);
-  } else row_barrier<NW>();
+      for (int w = 0; w < NW; w++) keys[w] = sh.key[w * 64 + t];
+      tau = kth_key<NW>(keys, top);
+      if (t == 0) sh.tau = tau;
+    }
+    __syncthreads();
+    tau = sh.tau;
+  } else {
+    const unsigned keys[1] = {order_key(lane_max)};
+    row_barrier<NW>();
+    tau = kth_key<1>(keys, top);
+  }
   const float bound = key_value(tau);
   unsigned long long mine = 0;      // which of the thread's elements are >= t
   if (lane_max >= bound)
@@ -85,12 +105,10 @@ __device__ inline void emit_top(V value, G fetch, float lane_max, int top, TopSh
   while (mine) {
     const int e = __builtin_ctzll(mine);
     mine &= mine - 1;
-    float v;
-    int c;
-    fetch(e, v, c);
+    const int c = column(e);
     if (c < 0) continue;
     const int slot = atomicAdd(&sh.count, 1);
-    if (slot < kCandidates) sh.cand[slot] = pair_key(v, c);
+    if (slot < kCandidates) sh.cand[slot] = pair_key(pick(e), c);
   }
   row_barrier<NW>();
   const int count = sh.count;
@@ -98,7 +116,9 @@ __device__ inline void emit_top(V value, G fetch, float lane_max, int top, TopSh
     for (int c = t; c < count; c += TPR) {
       const unsigned long long mine = sh.cand[c];
       int rank = 0;
-      for (int o = 0; o < count; o++) rank += sh.cand[o] > mine;
+      for (int o = 0; o < count; o += 8)      // (8 reads on their way together; what lies behind the last candidate does not count)
+#pragma unroll
+        for (int k = 0; k < 8; k++) rank += sh.cand[o + k] > mine && o + k < count ? 1 : 0;
       if (rank < top) emit(rank, key_value((unsigned)(mine >> 32)), (int)~(unsigned)mine);
     }
     for (int r = count + t; r < top; r += TPR) emit(r, -kInf, -1);
@@ -244,23 +264,30 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
   keep_packed<T, E>(v);
   if (m == -kInf) s = u = empty_sum<T, NW, E>(v, sh + 3 * NW);
   const auto value = [&](int i, int j) { return element<T>(v[i], j); };
-  const auto fetch = [&](int e, float &v, int &c) {
-    c = columns.column(e);
-    if (c < end) v = to_f32(z[c]);
-    else { v = -kInf; c = -1; }
+  const auto column = [&](int e) { const int c = columns.column(e); return c < end ? c : -1; };
+  const auto pick = [&](int e) {      // (a chain of selections: the elements' registers have no index)
+    const int word = sizeof(T) == 4 ? e : e / 2;
+    int w = v[0][0];
+#pragma unroll
+    for (int k = 1; k < E * 4; k++) w = word == k ? v[k / 4][k % 4] : w;
+    return element<T>(Packed{w, w, w, w}, e & 1);
   };
-  if (p.partial) {
-    if (t == 0) p.partial[item] = Partial{m, s, u, 0.0f};
-    if (p.top) emit_top<NW, E, N>(value, fetch, lane_max, p.top, top_sh[sub], [&](int rank, float value, int c) {
-      p.part_value[item * p.top + rank] = value;
-      p.part_col[item * p.top + rank] = c;
-    });
-    return;
+  const auto fetch = [&](int e, float &f, int &c) {
+    c = column(e);
+    f = c >= 0 ? to_f32(z[c]) : -kInf;
+  };
+  if (t == 0) {
+    if (p.partial) p.partial[item] = Partial{m, s, u, 0.0f};
+    else write_scores(p, row, m, s, u, has_label, label_value);
   }
-  if (t == 0) write_scores(p, row, m, s, u, has_label, label_value);
   if (p.top) {
     const float log_sum = logf(s);
-    emit_top<NW, E, N>(value, fetch, lane_max, p.top, top_sh[sub], [&](int rank, float value, int c) { write_alternative(p, row, rank, value, c, m, s, log_sum); });
+    emit_top<NW, E, N>(value, pick, column, fetch, lane_max, p.top, top_sh[sub], [&](int rank, float value, int c) {
+      if (p.partial) {
+        p.part_value[item * p.top + rank] = value;
+        p.part_col[item * p.top + rank] = c;
+      } else write_alternative(p, row, rank, value, c, m, s, log_sum);
+    });
   }
 }
 
@@ -297,12 +324,13 @@ template <typename T> __global__ __launch_bounds__(256) void k3_row_scores_join_
   if (threadIdx.x == 0) write_scores(p, row, m, s, u, has_label, label_value);
   if (p.top) {
     const float log_sum = logf(s);
-    const auto fetch = [&](int e, float &v, int &c) {
-      const int k = threadIdx.x + e * 256;
-      v = k < n ? p.part_value[first + k] : -kInf;
-      c = k < n ? p.part_col[first + k] : -1;
+    const auto column = [&](int e) { const int k = threadIdx.x + e * 256; return k < n ? p.part_col[first + k] : -1; };
+    const auto pick = [&](int e) { const int k = threadIdx.x + e * 256; return k < n ? p.part_value[first + k] : -kInf; };
+    const auto fetch = [&](int e, float &f, int &c) {
+      f = pick(e);
+      c = column(e);
     };
-    emit_top<4, E, 1>([&](int i, int) { return v[i]; }, fetch, lane_max, p.top, top_sh,
+    emit_top<4, E, 1>([&](int i, int) { return v[i]; }, pick, column, fetch, lane_max, p.top, top_sh,
                       [&](int rank, float value, int c) { write_alternative(p, row, rank, value, c, m, s, log_sum); });
   }
 }

@@ -13,12 +13,15 @@ template <typename T> struct Chunk { static constexpr int N = 16 / (int)sizeof(T
 
 template <typename T> __device__ inline float to_f32(T v) { return (float)v; }
 
-// chunk i of a row: `valid` elements of it exist (the rest is zero).  Rows end inside a chunk, never across one that is read past its end
+// The chunk at column col of a row of col + valid columns: `valid` elements of it exist (none: <= 0), the rest is zero.  Where the row ends inside it the elements are read one by one, all of
+// them, from addresses that stay in the row: loads under conditions would wait for each other.
 template <typename T> __device__ inline typename Chunk<T>::type load_chunk(const T *row, int col, int valid) {
   typename Chunk<T>::type v;
   if (valid >= Chunk<T>::N) return *reinterpret_cast<const typename Chunk<T>::type *>(row + col);
 #pragma unroll
-  for (int j = 0; j < Chunk<T>::N; j++) v[j] = j < valid ? row[col + j] : (T)0.0f;
+  for (int j = 0; j < Chunk<T>::N; j++) v[j] = row[min(col + j, col + valid - 1)];
+#pragma unroll
+  for (int j = 0; j < Chunk<T>::N; j++) v[j] = j < valid ? v[j] : (T)0.0f;
   return v;
 }
 template <typename T> __device__ inline void store_chunk(T *row, int col, int valid, typename Chunk<T>::type v) {
@@ -46,15 +49,17 @@ template <typename T> __device__ inline Packed load_packed(const T *row, int col
   Packed v;
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = __builtin_bit_cast(int, j < valid ? row[col + j] : otherwise);
+    for (int j = 0; j < 4; j++) {
+      const float e = row[min(col + j, col + valid - 1)];
+      v[j] = __builtin_bit_cast(int, j < valid ? e : otherwise);
+    }
   } else {
     const unsigned short fill = __builtin_bit_cast(unsigned short, otherwise);
-    const unsigned short *p = reinterpret_cast<const unsigned short *>(row) + col;
+    unsigned e[8];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const unsigned lo = 2 * j < valid ? p[2 * j] : fill, hi = 2 * j + 1 < valid ? p[2 * j + 1] : fill;
-      v[j] = (int)(lo | hi << 16);
-    }
+    for (int j = 0; j < 8; j++) e[j] = reinterpret_cast<const unsigned short *>(row)[min(col + j, col + valid - 1)];
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = (int)((2 * j < valid ? e[2 * j] : fill) | (2 * j + 1 < valid ? e[2 * j + 1] : fill) << 16);
   }
   return v;
 }
@@ -71,7 +76,9 @@ template <int N> __device__ inline void load_params(const float *p, int col, int
     return;
   }
 #pragma unroll
-  for (int j = 0; j < N; j++) out[j] = p && j < valid ? p[col + j] : otherwise;
+  for (int j = 0; j < N; j++) out[j] = p ? p[min(col + j, col + valid - 1)] : otherwise;
+#pragma unroll
+  for (int j = 0; j < N; j++) out[j] = j < valid ? out[j] : otherwise;
 }
 
 // lanes of a wavefront: inclusive combination over DPP row shifts and the two row broadcasts, complete in lane 63, in a fixed order
