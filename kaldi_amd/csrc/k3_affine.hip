@@ -181,7 +181,7 @@ template <int ROWS, int BK, bool ACROSS> struct Tile {
 template <typename T, int ROWS, int BK, bool ACROSS, int THREADS> struct Loader {
   using L = Tile<ROWS, BK, ACROSS>;
   static constexpr int N = L::kChunks / THREADS;
-  typedef T chunk __attribute__((ext_vector_type(8)));
+  typedef Packed chunk;
   const T *base; long long ld; int row0, rows, k;      // the operand, its first row in this tile, its number of rows, and the contraction's length
   int wave, lane;
   const char *from;      // uniform: where the next tile's offsets count from
@@ -211,11 +211,12 @@ template <typename T, int ROWS, int BK, bool ACROSS, int THREADS> struct Loader 
       int major, c;
       L::source((wave * N + i) * 64 + lane, major, c);
       const int row = ACROSS ? k0 + major : row0 + major, col = ACROSS ? row0 + c * 8 : k0 + c * 8, last = ACROSS ? rows : k;
-      const T *p = base + (long long)row * ld + col;
-      if (row < (ACROSS ? k : rows) && col + 8 <= last) v[i] = *(const u8 *)p;
-      else
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[i][j] = row < (ACROSS ? k : rows) && col + j < last ? p[j] : (T)0.0f;
+      const bool there = row < (ACROSS ? k : rows);      // (a row behind the last one: read from the first, and cleared)
+      const T *p = base + (there ? (long long)row * ld : 0);
+      Packed w;
+      if (last - col >= 8) w = __builtin_bit_cast(Packed, *(const u8 *)(p + col));
+      else w = load_packed<T>(p, col, last - col, (T)0.0f);
+      v[i] = there ? w : Packed{0, 0, 0, 0};
     }
   }
   __device__ inline void store(char *tile, const chunk (&v)[N]) const {
@@ -349,33 +350,43 @@ __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product
       __syncthreads();
     }
   }
-  // what is left of the contraction (everything, where the operands' alignment does not allow the direct way)
+  // what is left of the contraction (everything, where the operands' alignment does not allow the direct way): through registers, R tiles of them on their way
   if (direct < steps) {
-    typename LA::chunk va[LA::N];
-    typename LB::chunk vb[LB::N];
-    la.fetch(first + direct * BK, va);
-    lb.fetch(first + direct * BK, vb);
-    la.store(lds, va);
-    lb.store(lds + TA::kBytes, vb);
-    __syncthreads();
-    for (int s = direct; s < steps; s++) {
-      const int now = (s - direct) & 1;
-      if (s + 1 < steps) {
-        la.fetch(first + (s + 1) * BK, va);
-        lb.fetch(first + (s + 1) * BK, vb);
-      }
-      frag a[MI], b[NI];
+    constexpr int R = DIRECT || BM >= 128 ? 1 : 3;      // (two of 128 x 128 would leave a compute unit one workgroup instead of two)
+    typename LA::chunk va[R][LA::N];
+    typename LB::chunk vb[R][LB::N];
+    la.fetch(first + direct * BK, va[0]);
+    lb.fetch(first + direct * BK, vb[0]);
+    la.store(lds, va[0]);
+    lb.store(lds + TA::kBytes, vb[0]);
 #pragma unroll
-      for (int ks = 0; ks < 2; ks++) {
-        read(lds + now * kStage, ks, a, b);
-        multiply(a, b);
+    for (int r = 0; r < R; r++)
+      if (direct + 1 + r < steps) {
+        la.fetch(first + (direct + 1 + r) * BK, va[r]);
+        lb.fetch(first + (direct + 1 + r) * BK, vb[r]);
       }
-      if (s + 1 < steps) {
-        la.store(lds + (now ^ 1) * kStage, va);
-        lb.store(lds + (now ^ 1) * kStage + TA::kBytes, vb);
+    __syncthreads();
+    for (int s0 = direct; s0 < steps; s0 += R)
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const int s = s0 + r, now = (s - direct) & 1;
+        if (s >= steps) break;
+        frag a[MI], b[NI];
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+          read(lds + now * kStage, ks, a, b);
+          multiply(a, b);
+        }
+        if (s + 1 < steps) {
+          la.store(lds + (now ^ 1) * kStage, va[r]);
+          lb.store(lds + (now ^ 1) * kStage + TA::kBytes, vb[r]);
+          if (s + 1 + R < steps) {
+            la.fetch(first + (s + 1 + R) * BK, va[r]);
+            lb.fetch(first + (s + 1 + R) * BK, vb[r]);
+          }
+        }
+        __syncthreads();
       }
-      __syncthreads();
-    }
   }
   // The epilogue goes through LDS, a part of each wavefront's rows at a time (as many as its share of the tiles' memory holds): out of the accumulators' layout (4 columns of one of 16 rows
   // per lane) into runs of whole rows, so that what is read and written beside it are lines.  A row's chunk c of 4 lies at c ^ a function of the row that differs among the 16 rows that are
