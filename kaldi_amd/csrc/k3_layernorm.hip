@@ -10,6 +10,11 @@
 namespace {
 using namespace k3;
 
+// What the first mean m0 is off by, from the mean d and the mean square q of the differences from it.  The sum behind m0 is off by steps of the values' size, the one behind d by steps of
+// the differences': where the mean is large beside the spread, d is what the first sum lost (4096 +- 0.5 in float32: 1e-3 of the spread); otherwise it is noise, and the first sum (exact,
+// as a rule, for half-precision values) stays.
+__device__ inline float left_mean(float m0, float d, float q) { return m0 * m0 > 64.0f * q ? d : 0.0f; }
+
 // The rows a launch can hold in registers (up to 1024 threads of 16 or 24 elements).  A row belongs to NW wavefronts (one: four rows per workgroup); thread t holds the chunks t, t + 64 NW,
 // ... of it, E of them, so each element is read once and both sums of the forward pass run over registers.  A workgroup walks over rows with a stride of the whole launch: scale
 // and offset stay in registers, and the next row is on its way while this one is reduced and written.
@@ -56,7 +61,7 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
       }
     }
     block_sum2<NW>(d, q, sh + NW);
-    d /= n;      // what the rounding of the first mean left
+    d = left_mean(m0, d / n, q / n);
     const float r = 1.0f / sqrtf(fmaxf(q / n - d * d, 0.0f) + eps), m1 = m0 + d;
     if (t == 0) {
       if (mean) mean[row] = m1;
@@ -192,7 +197,7 @@ template <typename T> __global__ __launch_bounds__(256) void k3_ln_forward_loop_
   const float m0 = block_sum<4>(s, sh) / (float)cols;
   for (int c = threadIdx.x; c < cols; c += 256) { const float v = to_f32(xr[c]) - m0; d += v; q += v * v; }
   block_sum2<4>(d, q, sh + 4);
-  d /= (float)cols;      // what the rounding of the first mean left
+  d = left_mean(m0, d / (float)cols, q / (float)cols);
   const float r = 1.0f / sqrtf(fmaxf(q / (float)cols - d * d, 0.0f) + eps);
   if (threadIdx.x == 0) {
     if (mean) mean[row] = m0 + d;

@@ -13,17 +13,6 @@ template <typename T> struct Chunk { static constexpr int N = 16 / (int)sizeof(T
 
 template <typename T> __device__ inline float to_f32(T v) { return (float)v; }
 
-// The chunk at column col of a row of col + valid columns: `valid` elements of it exist (none: <= 0), the rest is zero.  Where the row ends inside it the elements are read one by one, all of
-// them, from addresses that stay in the row: loads under conditions would wait for each other.
-template <typename T> __device__ inline typename Chunk<T>::type load_chunk(const T *row, int col, int valid) {
-  typename Chunk<T>::type v;
-  if (valid >= Chunk<T>::N) return *reinterpret_cast<const typename Chunk<T>::type *>(row + col);
-#pragma unroll
-  for (int j = 0; j < Chunk<T>::N; j++) v[j] = row[min(col + j, col + valid - 1)];
-#pragma unroll
-  for (int j = 0; j < Chunk<T>::N; j++) v[j] = j < valid ? v[j] : (T)0.0f;
-  return v;
-}
 template <typename T> __device__ inline void store_chunk(T *row, int col, int valid, typename Chunk<T>::type v) {
   if (valid >= Chunk<T>::N) { *reinterpret_cast<typename Chunk<T>::type *>(row + col) = v; return; }
 #pragma unroll
@@ -43,26 +32,28 @@ template <typename T, int E> __device__ inline void keep_packed(Packed (&v)[E]) 
 #pragma unroll
     for (int i = 0; i < E; i++) asm volatile("" : "+v"(v[i]));
 }
-// a chunk of a row of which `valid` elements exist, `otherwise` behind them
+// The chunk at column col of a row of col + valid columns: `valid` elements of it exist (none: <= 0), `otherwise` stands behind them.  Where the row ends inside it, the row's last 16 bytes are
+// read and moved down: element by element it would be N loads instead of one, and under conditions they would wait for each other.
 template <typename T> __device__ inline Packed load_packed(const T *row, int col, int valid, T otherwise) {
-  if (valid >= Chunk<T>::N) return __builtin_bit_cast(Packed, *reinterpret_cast<const typename Chunk<T>::type *>(row + col));
-  Packed v;
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float e = row[min(col + j, col + valid - 1)];
-      v[j] = __builtin_bit_cast(int, j < valid ? e : otherwise);
+  constexpr int N = Chunk<T>::N, BITS = 8 * (int)sizeof(T);
+  typedef unsigned __int128 u128;
+  if (valid >= N) return __builtin_bit_cast(Packed, *reinterpret_cast<const typename Chunk<T>::type *>(row + col));
+  Packed fill;
+  if constexpr (sizeof(T) == 4) fill = Packed{1, 1, 1, 1} * __builtin_bit_cast(int, otherwise);
+  else fill = Packed{1, 1, 1, 1} * (int)(__builtin_bit_cast(unsigned short, otherwise) * 0x10001u);
+  if (valid <= 0) return fill;
+  u128 w;
+  if (col + valid >= N) w = __builtin_bit_cast(u128, *reinterpret_cast<const typename Chunk<T>::type *>(row + col + valid - N)) >> ((N - valid) * BITS);
+  else {      // (the whole row is shorter than a chunk)
+    w = 0;
+    for (int j = valid - 1; j >= 0; j--) {
+      if constexpr (sizeof(T) == 4) w = w << BITS | __builtin_bit_cast(unsigned, row[col + j]);
+      else w = w << BITS | __builtin_bit_cast(unsigned short, row[col + j]);
     }
-  } else {
-    const unsigned short fill = __builtin_bit_cast(unsigned short, otherwise);
-    unsigned e[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) e[j] = reinterpret_cast<const unsigned short *>(row)[min(col + j, col + valid - 1)];
-#pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = (int)((2 * j < valid ? e[2 * j] : fill) | (2 * j + 1 < valid ? e[2 * j + 1] : fill) << 16);
   }
-  return v;
+  return __builtin_bit_cast(Packed, w | (__builtin_bit_cast(u128, fill) & ~(u128)0 << (valid * BITS)));
 }
+template <typename T> __device__ inline typename Chunk<T>::type load_chunk(const T *row, int col, int valid) { return __builtin_bit_cast(typename Chunk<T>::type, load_packed<T>(row, col, valid, (T)0.0f)); }
 // N floats from a vector (null: `otherwise`)
 template <int N> __device__ inline void load_params(const float *p, int col, int valid, float otherwise, float *out) {
   typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
