@@ -577,14 +577,14 @@ int k3_layer_norm_backward(int32_t dtype, const void *d_x, int64_t ldx, const vo
                            void *d_dx, int64_t lddx, float *d_dscale, float *d_doffset, int32_t accumulate, void *d_workspace, int64_t workspace_bytes,
                            int32_t rows, int32_t cols, void *stream);
 /* An affine layer in half precision (dtype K3_F16 or K3_BF16): pre = x W^T + bias, y = act(pre) + residual, x [rows x inner], W [cols x inner] (AffineComponent's linear_params),
- * d_bias float32 [cols] (null: 0), d_residual [rows x cols] (null: none; y may be it).  d_pre (null: not kept) receives pre as the backward pass takes it.  Products are summed in float32 and
+ * d_bias float32 [cols] (null: 0), d_residual [rows x cols] (null: none; y may be it, and no other matrix).  d_pre (null: not kept) receives pre as the backward pass takes it.  Products are summed in float32 and
  * a result is rounded once.  Stands beside k3_mat_add_mat_mat, which is float32 and has no epilogue.  Workspace (16-byte aligned): k3_affine_forward_workspace. */
 typedef enum { K3_ACT_NONE = 0, K3_ACT_RELU = 1, K3_ACT_SIGMOID = 2, K3_ACT_TANH = 3, K3_ACT_SWISH = 4 /* z sigmoid(z) */, K3_ACT_GELU = 5 /* z (1 + erf(z / sqrt 2)) / 2 */ } k3_activation;
 int64_t k3_affine_forward_workspace(int32_t rows, int32_t inner, int32_t cols);
 int k3_affine_forward(int32_t dtype, int32_t act, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const float *d_bias, const void *d_residual, int64_t ldr, void *d_y,
                       int64_t ldy, void *d_pre, int64_t ldp, void *d_workspace, int64_t workspace_bytes, int32_t rows, int32_t inner, int32_t cols, void *stream);
 /* Its derivatives from dy: dz = dy act'(pre) (d_pre not read for K3_ACT_NONE), d_dx = dz W and d_dw = dz^T x (of the matrices' type), d_db [cols] = the sum of dz over the rows (float32);
- * each may be null (not wanted), and what is given is overwritten.  (The residual's derivative is dy itself.)  Where there is an activation, dz is rounded to the matrices' type for the two
+ * each may be null (not wanted), and what is given is overwritten and lies on no input.  (The residual's derivative is dy itself.)  Where there is an activation, dz is rounded to the matrices' type for the two
  * products, not for d_db.  Sums are taken in a fixed order.  rows = 0 clears d_dw and d_db.  Workspace (16-byte aligned): k3_affine_backward_workspace. */
 int64_t k3_affine_backward_workspace(int32_t act, int32_t rows, int32_t inner, int32_t cols);
 int k3_affine_backward(int32_t dtype, int32_t act, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_pre, int64_t ldp, const void *d_dy, int64_t lddy,
@@ -594,12 +594,13 @@ int k3_affine_backward(int32_t dtype, int32_t act, const void *d_x, int64_t ldx,
  * the matrix of log-probabilities.  d_labels [rows] (a label outside 0 .. cols - 1, -1 for instance, = none: its log-probability is 0); every output may be null: d_log_prob, d_entropy
  * [rows]; d_stats [rows][2] = the row's largest value and ln sum exp(z - it), which the derivative takes; d_alt_log_probs, d_alt_labels [rows][num_alternatives].
  * -inf in z = a column that cannot be (probability 0).  A row of nothing but -inf has log-probabilities -inf and entropy 0; one that holds a NaN or +inf has NaN scores and no
- * alternatives (-1).  At most 2^21 columns.  Workspace (16-byte aligned, may be null where 0 bytes are asked for): k3_label_logprobs_workspace. */
+ * alternatives (-1).  At most 2^19 columns.  Workspace (16-byte aligned, may be null where 0 bytes are asked for): k3_label_logprobs_workspace. */
 int64_t k3_label_logprobs_workspace(int32_t dtype, int32_t rows, int32_t cols, int32_t num_alternatives);
 int k3_label_logprobs(int32_t dtype, const void *d_z, int64_t ld, const int32_t *d_labels, float *d_log_prob, float *d_entropy, float *d_stats, int32_t num_alternatives,
                       float *d_alt_log_probs, int32_t *d_alt_labels, void *d_workspace, int64_t workspace_bytes, int32_t rows, int32_t cols, void *stream);
 /* The derivative of sum_r d_log_prob_deriv[r] log q_y(r) + d_entropy_deriv[r] entropy(r) with respect to z, into d_dz (overwritten; may be z).  d_stats (and d_entropy, where
- * d_entropy_deriv is given) are the forward pass's; either derivative may be null (0); a row without a label has no first term; a row of nothing but -inf gets zeros. */
+ * d_entropy_deriv is given) are the forward pass's; either derivative may be null (0); a row without a label has no first term; a row of
+ * nothing but -inf gets zeros, and so does one whose two derivatives are 0, whatever it holds. */
 int k3_label_logprobs_deriv(int32_t dtype, const void *d_z, int64_t ld, const int32_t *d_labels, const float *d_stats, const float *d_entropy, const float *d_log_prob_deriv,
                             const float *d_entropy_deriv, void *d_dz, int64_t ldd, int32_t rows, int32_t cols, void *stream);
 /* Distillation from a teacher's top logits: row r has num_entries (1 .. 1024) pairs of a teacher value (of z's type) and its column; a column outside 0 .. cols - 1, -1 for instance =
@@ -607,7 +608,7 @@ int k3_label_logprobs_deriv(int32_t dtype, const void *d_z, int64_t ld, const in
  *   d_objf[r] = w_r T^2 sum_k p_k (log q_{i_k} - log p_k)      (the negative divergence of p from q: to be maximised, as the chain objective is)
  *   d_dz[r][j] = w_r T (sum of p_k over i_k = j  -  q_j)       (its derivative; overwritten, may be z; d_dz null: not wanted)
  * A column may come more than once.  d_weights [rows] (null: 1).  A row without a used entry (or with nothing but -inf in them), or of weight 0, has objective 0 and zeros, whatever z
- * holds; otherwise a row of z with nothing but -inf has objective -inf w_r and zeros.  One entry per row is the cross entropy.  At most 2^21 columns.
+ * holds; otherwise a row of z with nothing but -inf has objective -inf w_r and zeros.  One entry per row is the cross entropy.  At most 2^19 columns.
  * Workspace (16-byte aligned, may be null where 0 bytes are asked for): k3_distill_workspace. */
 int64_t k3_distill_workspace(int32_t dtype, int32_t rows, int32_t cols, int32_t num_entries, int32_t with_deriv);
 int k3_distill_objf_and_deriv(int32_t dtype, float temperature, const void *d_z, int64_t ld, const void *d_teacher_values, int64_t ld_values, const int32_t *d_teacher_indexes,

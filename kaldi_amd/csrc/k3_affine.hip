@@ -587,7 +587,8 @@ template <typename T, bool A_ACROSS, bool B_ACROSS> int run_product(Product p, v
 
 constexpr int kMaxStrips = 256;
 constexpr int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
-bool sizes_ok(int rows, int inner, int cols) { return (int64_t)rows * ((int64_t)inner + cols) < (1ll << 42) && inner <= (1 << 20) && cols <= (1 << 22); }
+bool sizes_ok(int rows, int inner, int cols) { return rows <= 1 << 30 && (int64_t)rows * ((int64_t)inner + cols) < (1ll << 42) && inner <= (1 << 20) && cols <= (1 << 22); }
+int64_t sums_bytes(int rows, int cols) { return up256((int64_t)std::min((rows + 3) / 4, kMaxStrips) * cols * 4); }      // of the slope kernel: a strip is 4 rows at least
 
 template <typename T> int affine_forward(Product p, void *workspace, hipStream_t st) { return run_product<T, false, false>(p, workspace, st); }
 struct Backward { const void *x; long long ldx; const void *w; long long ldw; const void *pre; long long ldp; const void *dy; long long lddy; void *dx; long long lddx; void *dw; long long lddw;
@@ -605,7 +606,7 @@ template <typename T> int affine_backward(const Backward &q, char *workspace, hi
       lddz = (q.cols + 7) / 8 * 8;
       rest += up256((int64_t)q.rows * lddz * 2);
     }
-    if (q.db) { partial = (float *)rest; rest += up256((int64_t)kMaxStrips * q.cols * 4); }
+    if (q.db) { partial = (float *)rest; rest += sums_bytes(q.rows, q.cols); }
     // enough strips to fill the chip, of a row per wavefront at least; a single one writes the sums at their place
     const int across = (q.cols + 511) / 512, least = (q.rows + kMaxStrips - 1) / kMaxStrips;
     const int strip = std::max({4, least, (int)((long long)q.rows * across / 2048)}), strips = (q.rows + strip - 1) / strip;
@@ -647,6 +648,7 @@ extern "C" int k3_affine_forward(int32_t dtype, int32_t act, const void *d_x, in
   if (!sizes_ok(rows, inner, cols)) { set_error("k3_affine_forward: matrix too large"); return K3_ERR_UNSUPPORTED; }
   if (rows == 0) return K3_OK;
   K3_REQUIRE(d_x && d_w && d_y, "k3_affine_forward: null matrix");
+  K3_REQUIRE(d_y != d_x && d_y != d_w && d_y != d_pre && (!d_pre || (d_pre != d_x && d_pre != d_w && d_pre != d_residual)), "k3_affine_forward: an output lies on another matrix");
   K3_REQUIRE(workspace_bytes >= k3_affine_forward_workspace(rows, inner, cols) && (d_workspace || workspace_bytes == 0) && ((uintptr_t)d_workspace & 15) == 0,
              "k3_affine_forward: workspace too small or not aligned");
   Product p{};
@@ -657,7 +659,7 @@ extern "C" int k3_affine_forward(int32_t dtype, int32_t act, const void *d_x, in
 
 extern "C" int64_t k3_affine_backward_workspace(int32_t act, int32_t rows, int32_t inner, int32_t cols) {
   if (rows <= 0 || inner <= 0 || cols <= 0 || !sizes_ok(rows, inner, cols)) return 0;
-  return (act == kNone ? 0 : up256((int64_t)rows * ((cols + 7) / 8 * 8) * 2)) + up256((int64_t)kMaxStrips * cols * 4) +
+  return (act == kNone ? 0 : up256((int64_t)rows * ((cols + 7) / 8 * 8) * 2)) + sums_bytes(rows, cols) +
          std::max(plan_product(rows, inner, cols).bytes, plan_product(cols, inner, rows).bytes);
 }
 
@@ -670,6 +672,9 @@ extern "C" int k3_affine_backward(int32_t dtype, int32_t act, const void *d_x, i
              "k3_affine_backward: bad argument");
   if (!sizes_ok(rows, inner, cols)) { set_error("k3_affine_backward: matrix too large"); return K3_ERR_UNSUPPORTED; }
   K3_REQUIRE(rows == 0 || (d_dy && (d_x || !d_dw) && (d_w || !d_dx) && (d_pre || act == kNone)), "k3_affine_backward: null input");
+  for (const void *out : {(const void *)d_dx, (const void *)d_dw})
+    K3_REQUIRE(!out || rows == 0 || (out != d_x && out != d_w && out != d_dy && (act == kNone || out != d_pre)), "k3_affine_backward: an output lies on an input");
+  K3_REQUIRE(!d_dx || d_dx != d_dw, "k3_affine_backward: the outputs lie on each other");
   K3_REQUIRE(workspace_bytes >= k3_affine_backward_workspace(act, rows, inner, cols) && (d_workspace || workspace_bytes == 0) && ((uintptr_t)d_workspace & 15) == 0,
              "k3_affine_backward: workspace too small or not aligned");
   const Backward q{d_x, ldx, d_w, ldw, d_pre, ldp, d_dy, lddy, rows ? d_dx : nullptr, lddx, d_dw, lddw, d_db, act, rows, inner, cols};

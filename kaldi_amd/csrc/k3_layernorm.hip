@@ -307,7 +307,7 @@ template <typename T> void forward(const void *x, long long ldx, const float *sc
   }
   with_shape<T>(s, [&](auto nw, auto e) {
     constexpr int NW = decltype(nw)::value, E = decltype(e)::value, RPB = NW == 1 ? 4 : 1;
-    const int grid = std::min((rows + RPB - 1) / RPB, 256 * (NW <= 4 ? 16 / std::max(NW, 4) * 2 : 16 / NW * 2));
+    const int grid = std::min((rows - 1) / RPB + 1, 256 * (NW <= 4 ? 16 / std::max(NW, 4) * 2 : 16 / NW * 2));
     hipLaunchKernelGGL((k3_ln_forward_kernel<T, NW, E>), dim3(grid), dim3(NW == 1 ? 256 : 64 * NW), 0, st, (const T *)x, ldx, scale, offset, eps, (T *)y, ldy, mean, inv_std, rows, cols);
   });
 }
@@ -326,7 +326,7 @@ template <typename T> int backward(const void *x, long long ldx, const void *dy,
   int grid = 0;
   with_shape<T>(s, [&](auto nw, auto e) {
     constexpr int NW = decltype(nw)::value, E = decltype(e)::value, RPB = NW == 1 ? 4 : 1;
-    grid = std::min((rows + RPB - 1) / RPB, NW <= 8 ? kMaxStrips : kMaxStrips / 2);
+    grid = std::min((rows - 1) / RPB + 1, NW <= 8 ? kMaxStrips : kMaxStrips / 2);
     hipLaunchKernelGGL((k3_ln_backward_kernel<T, NW, E>), dim3(grid), dim3(NW == 1 ? 256 : 64 * NW), 0, st, (const T *)x, ldx, (const T *)dy, lddy, scale, mean, inv_std, (T *)dx, lddx,
                        partial, rows, cols);
   });
@@ -349,7 +349,7 @@ extern "C" int k3_layer_norm_forward(int32_t dtype, const void *d_x, int64_t ldx
 
 extern "C" int64_t k3_layer_norm_backward_workspace(int32_t rows, int32_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return (int64_t)sizeof(float) * 2 * cols * kMaxStrips;
+  return (int64_t)sizeof(float) * 2 * cols * std::min(rows, kMaxStrips);
 }
 
 extern "C" int k3_layer_norm_backward(int32_t dtype, const void *d_x, int64_t ldx, const void *d_dy, int64_t lddy, const float *d_scale, const float *d_mean, const float *d_inv_std,

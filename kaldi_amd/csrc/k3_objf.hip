@@ -350,7 +350,7 @@ template <typename T> __global__ __launch_bounds__(256) void k3_label_deriv_kern
   int y = labels ? labels[row] : -1;
   if (y < 0 || y >= cols) y = -1;
   const float g = y >= 0 && log_prob_deriv ? log_prob_deriv[row] : 0.0f, b = -h, c = -g - (h != 0.0f ? h * entropy[row] : 0.0f);
-  const bool empty = m == -kInf;
+  const bool empty = m == -kInf || (g == 0.0f && h == 0.0f);      // (nothing to pass on: zeros, whatever the row holds)
   columns.store(dz + row * ldd, v, [&](Packed w, int e, int j) {
     const float lq = element<T>(w, j) - m - log_sum, q = exp2_fast(lq * kLog2e), d = q * __builtin_fmaf(b, fmaxf(lq, -16384.0f), c);      // (q = 0 where lq = -inf)
     return empty ? 0.0f : columns.column(e) == y ? d + g : d;
@@ -590,7 +590,7 @@ template <typename T> int distill(DistillArgs p, void *workspace, hipStream_t st
   if (s.e) {
     const auto launch = [&](auto nw, auto e) {
       constexpr int NW = decltype(nw)::value, E = decltype(e)::value, RPB = NW == 1 ? 4 : 1;
-      hipLaunchKernelGGL((k3_distill_kernel<T, NW, E>), dim3((unsigned)((p.rows + RPB - 1) / RPB)), dim3(NW == 1 ? 256 : 64 * NW), sizeof(Entry) * RPB * p.top, st, p);
+      hipLaunchKernelGGL((k3_distill_kernel<T, NW, E>), dim3((unsigned)((p.rows - 1) / RPB + 1)), dim3(NW == 1 ? 256 : 64 * NW), sizeof(Entry) * RPB * p.top, st, p);
     };
     if (s.nw == 1) with_chunks<1>(s.e, launch);
     else if (s.nw == 4) with_chunks<4>(s.e, launch);
@@ -622,7 +622,7 @@ template <typename T> int distill(DistillArgs p, void *workspace, hipStream_t st
   return K3_OK;
 }
 
-const int kMaxCols = 1 << 21;      // 64 parts of what a workgroup of four wavefronts holds of float32 columns, rounded to their granule, hold a row of that many
+const int kMaxCols = kMaxSplits * 4 * 64 * 8 * 4;      // 64 parts of what a workgroup of four wavefronts holds of float32 columns: 2^19
 
 }  // namespace
 

@@ -136,6 +136,25 @@ def test_distillation_matches_the_formulas(rows, cols, dtype):
         assert_within(o2, want, e * mag + e * T * T * ww.abs() + 1e-30, "objf alone")
         ComputeDistillObjfAndDeriv(DistillationOptions(T), z, t, idx, w, o2, z); assert torch.equal(z, dz) and torch.equal(o2, objf)      # in place
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_widest_rows(dtype):
+    """2^19 columns, the last of them the label, an alternative and a teacher's entry: every part of the row comes in"""
+    from kaldi_amd.objective import LabelLogProbs, DiffLabelLogProbs, ComputeDistillObjfAndDeriv, DistillationOptions
+    rows, cols = 3, 1 << 19; g = generator(19); z = torch.randn(rows, cols, generator=g, device="cuda").to(dtype); z[:, -1] = 9.0; z[:, 0] = 8.0; z[1, cols // 2 + 1] = 10.0
+    y = torch.full((rows,), cols - 1, dtype=torch.int32, device="cuda"); lp, h, st = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty(rows, 2, device="cuda"); al, ai = torch.empty(rows, 40, device="cuda"), torch.empty(rows, 40, dtype=torch.int32, device="cuda")
+    LabelLogProbs(z, y, lp, h, st, al, ai); m, ls, lq, q, H = scores64(z); e = S(cols, 40) + 8 * U32 * ls; idx = best64(z, 40)
+    assert_within(lp, lq[:, -1], e, "log prob"); assert_within(h, H, e + S(cols, 40) * (H + ls), "entropy"); assert torch.equal(ai.long(), idx); assert_within(al, lq.gather(1, idx), e[:, None].expand(rows, 40), "alternatives")
+    t = torch.tensor([[1.0, 0.0]], device="cuda").expand(rows, 2).contiguous().to(dtype); ti = torch.tensor([[cols - 1, 5]], dtype=torch.int32, device="cuda").expand(rows, 2).contiguous(); f, dz = torch.empty(rows, device="cuda"), torch.empty_like(z)
+    ComputeDistillObjfAndDeriv(DistillationOptions(), z, t, ti, None, f, dz); want, d, _, _, _, _ = distill64(z, t, ti, torch.ones(rows, device="cuda"), 1.0)
+    assert_within(f, want, S(cols, 40) * 40 * torch.ones_like(want), "objf"); off = S(cols, 40) * (q + d.abs()) + S(cols, 40) * (d > 0); assert_within(dz, d, half_step(dtype) * (d.abs() + off) + off + (2.0 ** -25 if dtype == torch.float16 else 0.0), "dz")
+
+def test_rows_with_nothing_to_pass_on_get_zeros():
+    """padding with NaNs and infinities in it, no label and no derivative of the entropy: zeros"""
+    from kaldi_amd.objective import LabelLogProbs, DiffLabelLogProbs
+    for cols in (100, 5000):
+        z = torch.randn(4, cols, generator=generator(cols), device="cuda"); z[1, 3] = float("nan"); z[2] = float("inf"); y = torch.tensor([1, -1, -1, 2], dtype=torch.int32, device="cuda"); h, st = torch.empty(4, device="cuda"), torch.empty(4, 2, device="cuda"); LabelLogProbs(z, y, None, h, st)
+        dz = torch.empty_like(z); DiffLabelLogProbs(z, y, st, None, torch.ones(4, device="cuda"), None, dz); assert (dz[1:3] == 0).all() and torch.isfinite(dz).all() and dz[0, 1] > 0 and dz[3, 2] > 0
+
 def test_distillation_edges():
     from kaldi_amd.objective import ComputeDistillObjfAndDeriv, DistillationOptions
     inf = float("inf"); o = DistillationOptions()

@@ -25,7 +25,7 @@ def test_label_entry_points():
     L = _l.load()
     f = lambda dtype=0, z=P, ld=8, y=P, lp=P, n=0, al=None, ai=None, ws=None, nb=0, rows=4, cols=8: L.k3_label_logprobs(dtype, z, ld, y, lp, None, None, n, al, ai, ws, nb, rows, cols, None)  # noqa: E731
     refused(f(dtype=3), "type"); refused(f(ld=7), "bad argument"); refused(f(rows=-1), "bad argument"); refused(f(cols=0), "bad argument"); refused(f(n=-1), "bad argument"); refused(f(z=None), "null"); refused(f(y=None), "null")
-    refused(f(n=65, al=P, cols=100, ld=100), "at most"); refused(f(cols=(1 << 21) + 1, ld=1 << 22), "at most"); refused(f(n=9, al=P), "more alternatives"); refused(f(n=3), "do not go together"); refused(f(al=P), "do not go together")
+    refused(f(n=65, al=P, cols=100, ld=100), "at most"); refused(f(cols=(1 << 19) + 1, ld=1 << 22), "at most"); refused(f(n=9, al=P), "more alternatives"); refused(f(n=3), "do not go together"); refused(f(al=P), "do not go together")
     assert f(rows=0) == 0
     need = L.k3_label_logprobs_workspace(0, 4, 100000, 5); assert need > 0 and L.k3_label_logprobs_workspace(0, 4000, 6024, 5) == 0
     refused(f(cols=100000, ld=100000, n=5, al=P, ws=P, nb=need - 1), "workspace"); refused(f(cols=100000, ld=100000, n=5, al=P, ws=P + 4, nb=need), "workspace"); refused(f(cols=100000, ld=100000, n=5, al=P), "workspace")
@@ -40,7 +40,7 @@ def test_distillation_entry_point():
     refused(f(dtype=3), "type")
     for T in (0.0, -1.0, float("nan"), float("inf"), 1e-4): refused(f(T=T), "temperature")
     for k in ("ld", "ldv", "ldi", "ldd"): refused(f(**{k: 2}), "bad argument")
-    refused(f(n=0), "bad argument"); refused(f(cols=0), "bad argument"); refused(f(rows=-1), "bad argument"); refused(f(n=1025, ldv=2000, ldi=2000), "at most"); refused(f(cols=(1 << 21) + 1, ld=1 << 22, ldd=1 << 22), "at most")
+    refused(f(n=0), "bad argument"); refused(f(cols=0), "bad argument"); refused(f(rows=-1), "bad argument"); refused(f(n=1025, ldv=2000, ldi=2000), "at most"); refused(f(cols=(1 << 19) + 1, ld=1 << 22, ldd=1 << 22), "at most")
     for k in ("z", "v", "i", "o"): refused(f(**{k: None}), "null")
     assert f(rows=0) == 0
     need = L.k3_distill_workspace(0, 4, 200000, 3, 1); assert need > 0 and L.k3_distill_workspace(0, 4, 6024, 3, 1) == 0
@@ -49,7 +49,7 @@ def test_distillation_entry_point():
 def test_affine_entry_points():
     L = _l.load()
     need = L.k3_affine_forward_workspace(4, 4096, 8); assert need > 0
-    f = lambda dtype=1, act=0, x=P, ldx=4096, w=P, ldw=4096, r=None, ldr=8, y=P, ldy=8, pre=None, ldp=8, ws=P, n=need, rows=4, inner=4096, cols=8: L.k3_affine_forward(dtype, act, x, ldx, w, ldw, None, r, ldr, y, ldy, pre, ldp, ws, n, rows, inner, cols, None)  # noqa: E731
+    f = lambda dtype=1, act=0, x=P, ldx=4096, w=2 * P, ldw=4096, r=None, ldr=8, y=3 * P, ldy=8, pre=None, ldp=8, ws=P, n=need, rows=4, inner=4096, cols=8: L.k3_affine_forward(dtype, act, x, ldx, w, ldw, None, r, ldr, y, ldy, pre, ldp, ws, n, rows, inner, cols, None)  # noqa: E731
     for d in (0, 3, -1): refused(f(dtype=d), "float16 and bfloat16")
     refused(f(act=6), "activation"); refused(f(act=-1), "activation")
     for k in ("ldx", "ldw", "ldy"): refused(f(**{k: 7}), "bad argument")
@@ -57,13 +57,16 @@ def test_affine_entry_points():
     refused(f(inner=1 << 21, ldx=1 << 21, ldw=1 << 21), "too large"); refused(f(rows=(1 << 31) - 1, cols=4096, ldy=4096), "too large")
     for k in ("x", "w", "y"): refused(f(**{k: None}), "null")
     refused(f(ws=None), "workspace"); refused(f(n=need - 1), "workspace"); refused(f(ws=P + 4), "workspace"); assert f(rows=0) == 0
+    for k in (dict(y=P), dict(y=2 * P), dict(pre=3 * P), dict(pre=P), dict(pre=2 * P), dict(pre=5 * P, r=5 * P)): refused(f(**k), "lies on")
     need = L.k3_affine_backward_workspace(1, 4, 4096, 8); assert need > 0
-    b = lambda dtype=1, act=1, x=P, ldx=4096, w=P, ldw=4096, pre=P, ldp=8, dy=P, lddy=8, dx=P, lddx=4096, dw=P, lddw=4096, ws=P, n=need, rows=4, inner=4096, cols=8: L.k3_affine_backward(dtype, act, x, ldx, w, ldw, pre, ldp, dy, lddy, dx, lddx, dw, lddw, P, ws, n, rows, inner, cols, None)  # noqa: E731
+    b = lambda dtype=1, act=1, x=P, ldx=4096, w=2 * P, ldw=4096, pre=3 * P, ldp=8, dy=4 * P, lddy=8, dx=5 * P, lddx=4096, dw=6 * P, lddw=4096, ws=P, n=need, rows=4, inner=4096, cols=8: L.k3_affine_backward(dtype, act, x, ldx, w, ldw, pre, ldp, dy, lddy, dx, lddx, dw, lddw, P, ws, n, rows, inner, cols, None)  # noqa: E731
     refused(b(dtype=0), "float16 and bfloat16"); refused(b(act=9), "activation")
     for k in ("ldx", "ldw", "ldp", "lddy", "lddx", "lddw"): refused(b(**{k: 7}), "bad argument")
     refused(b(rows=-1), "bad argument"); refused(b(inner=0), "bad argument"); refused(b(cols=0), "bad argument"); refused(b(inner=1 << 21, ldx=1 << 21, ldw=1 << 21, lddx=1 << 21, lddw=1 << 21), "too large")
     for k in ("x", "w", "pre", "dy"): refused(b(**{k: None}), "null")
     refused(b(ws=None), "workspace"); refused(b(n=need - 1), "workspace"); refused(b(ws=P + 4), "workspace")
+    for at in (1, 2, 3, 4): refused(b(dx=at * P), "lies on"); refused(b(dw=at * P), "lies on")
+    refused(b(dw=5 * P), "lie on each other")
 
 def test_matrices_that_are_no_rows_on_a_gpu():
     from kaldi_amd import cumatrix as cm, objective as ob
