@@ -3,6 +3,8 @@
 //   backward, with xhat = (x - mean) inv_std and g = dy scale:  dx = inv_std (g - mean(g) - xhat mean(g xhat)), dscale = sum over rows of dy xhat, doffset = sum over rows of dy
 // The reference has the norm without a mean (NormalizeComponent, cudamatrix/cu-math.h:272-300; k3_mat_normalize_rows here) and no half-precision matrices.
 // All sums are kept in float32; a value is rounded to the matrix's type once, when it is written.
+// Bound by memory: 2 (forward) or 3 (backward) passes over the matrix and nothing else of its size.  Measured: float16 40011 x 1535 forward 55 us (4.5 TB/s, rows that start anywhere),
+// bfloat16 32768 x 4096 backward 151 us (5.3 TB/s; a copy of 1 GB runs at 5.0).
 #include "k3_rowops.h"
 #include <algorithm>
 #include <type_traits>
