@@ -4,8 +4,8 @@
 // All three products are C[m][n] = sum_k A(m, k) B(n, k) on the matrix cores (16 x 16 x 32, float32 accumulation); an operand's contraction index is its contiguous one (x, W, dz for dx) or
 // its row index (W for dx; dz and x for dW).  The former is read from LDS as it lies (16 bytes of one row per lane), the latter with the transposing LDS read (4 contraction steps of
 // 16 rows per 16 lanes), so no operand is ever transposed in memory.
-// Measured in bfloat16: 8192 x 8192 x 8192 952 us forward (1.15 PFLOP/s), 1020 dx, 945 dW; 42752 x 1536 x 1536 with ReLU, bypass and the activation's input kept 237 us (197 without them: the
-// epilogues of all compute units come at the same time); 25600 x 768 x 6024 286 us dx, 285 dW (its rows of 12048 bytes straddle cache lines; the matrix cores are busy a third of the time).
+// Measured in bfloat16: 8192 x 8192 x 8192 948 us forward (1.16 PFLOP/s), 1028 dx, 934 dW; 42752 x 1536 x 1536 with ReLU, bypass and the activation's input kept 236 us (198 without them: the
+// epilogues of all compute units come at the same time); 25600 x 768 x 6024 292 us dx, 290 dW (matrix cores busy 35 % of the cycles by counters; its rows of 12048 bytes straddle cache lines).
 #include "k3_rowops.h"
 #include <algorithm>
 #include <type_traits>

@@ -4,9 +4,9 @@
 //   distillation, p = softmax of a row's teacher values:  objf = w T^2 sum_k p_k (log q_{i_k} - log p_k),  d objf / d z_j = w T (sum of p_k over i_k = j  -  q_j)
 // Elements are held as they are stored and widened where they are used; statistics, sums and exponentials are float32.  The difference is taken before the product: a z_j alone would
 // overflow at the lowest values of float32 and bfloat16, which masks are made of.
-// Bound by memory, a row being read once (and its derivative written once): scores of float32 42752 x 6024 with 4 alternatives 166 us (6.2 TB/s), label derivative of bfloat16 2000 x 50001
-// 78 us (5.1), distillation with derivative of float32 6400 x 6024 66 us (4.7) and of bfloat16 4096 x 128000 505 us (4.2: a row fills a compute unit's registers, and its
-// exponentials, 17 us a row, run under its own loads and stores only in part).
+// Bound by memory, a row being read once (and its derivative written once): scores of float32 42752 x 6024 with 4 alternatives 168 us (6.1 TB/s), label derivative of bfloat16 2000 x 50001
+// 78 us (5.1), distillation with derivative of float32 6400 x 6024 67 us (4.6) and of bfloat16 4096 x 128000 508 us (4.1: a row fills a compute unit's registers, and its
+// vector instructions, 54 % of the cycles by counters, run under its own loads and stores only in part).
 #include "k3_rowops.h"
 #include <algorithm>
 #include <type_traits>
