@@ -5,7 +5,7 @@
 // its row index (W for dx; dz and x for dW).  The former is read from LDS as it lies (16 bytes of one row per lane), the latter with the transposing LDS read (4 contraction steps of
 // 16 rows per 16 lanes), so no operand is ever transposed in memory.
 // Measured in bfloat16: 8192 x 8192 x 8192 948 us forward (1.16 PFLOP/s), 1028 dx, 934 dW; 42752 x 1536 x 1536 with ReLU, bypass and the activation's input kept 236 us (198 without them: the
-// epilogues of all compute units come at the same time); 25600 x 768 x 6024 292 us dx, 290 dW (matrix cores busy 35 % of the cycles by counters; its rows of 12048 bytes straddle cache lines).
+// epilogues of all compute units come at the same time); 25600 x 768 x 6024 292 us dx, 290 dW (matrix cores busy 35 % of the chip's cycles by counters; its rows of 12048 bytes straddle cache lines).
 #include "k3_rowops.h"
 #include <algorithm>
 #include <type_traits>
@@ -239,8 +239,8 @@ __device__ inline void place(const Product &p, int tile, int &tm, int &tn) {
 }
 
 // BM x BN outputs per workgroup of WM x WN wavefronts, over LDS tiles of 64 contraction steps, two of them: one is loaded while the other is multiplied.  PIPED (the size of which a compute
-// unit holds one workgroup): a tile is two halves of 32 steps for the matrix instructions, and the fragments of a half are read from LDS among the instructions of the half before it, those of the next tile's first half too: the one barrier per
-// tile stands between the halves, where every wavefront has read all of this tile (which the loads issued behind the barrier then overwrite) and the next one has arrived.
+// unit holds one workgroup): a tile is two halves of 32 steps for the matrix instructions, and the fragments of a half are read from LDS among the instructions of the half before it, those
+// of the next tile's first half too: the one barrier per tile stands between the halves, where every wavefront has read all of this tile (which the loads issued behind the barrier then overwrite) and the next one has arrived.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_ACROSS, bool B_ACROSS, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product p) {
   constexpr int THREADS = 64 * WM * WN, MI = BM / WM / 16, NI = BN / WN / 16, BK = 64;
@@ -259,174 +259,174 @@ __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product
   const long long run_end = split ? p.run_start(unit + 1) : 0;
   long long at = split ? p.run_start(unit) : 0;
   do {      // one round per piece of a tile: this workgroup's tile, or what its run has of one
-  const int t = split ? (int)(at / p.steps) : 0, step0 = split ? (int)(at - (long long)t * p.steps) : 0, step1 = split ? (int)min((long long)p.steps, step0 + run_end - at) : p.steps;
-  const bool piece = step0 > 0 || step1 < p.steps;
-  at += step1 - step0;
-  int thread = threadIdx.x;
-  asm volatile("" : "+v"(thread));      // (what is made of it is made anew for every piece, and takes no registers from the loop below)
-  const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), wm = wave / WN, wn = wave % WN;
-  int tm, tn;
-  place(p, split ? p.whole + t : unit, tm, tn);
-  const int first = step0 * BK, end = min(p.k, step1 * BK);
-  const int direct = DIRECT ? (end - first) / BK : 0, steps = (end - first + BK - 1) / BK;
-  LA la{(const T *)p.a, p.lda, tm * BM, p.m, p.k, wave, lane};
-  LB lb{(const T *)p.b, p.ldb, tn * BN, p.n, p.k, wave, lane};
-  f4 acc[MI][NI] = {};
-  typedef typename Half<T>::frag frag;
-  const auto read = [&](const char *ta, int ks, frag (&a)[MI], frag (&b)[NI]) {
+    const int t = split ? (int)(at / p.steps) : 0, step0 = split ? (int)(at - (long long)t * p.steps) : 0, step1 = split ? (int)min((long long)p.steps, step0 + run_end - at) : p.steps;
+    const bool piece = step0 > 0 || step1 < p.steps;
+    at += step1 - step0;
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));      // (what is made of it is made anew for every piece, and takes no registers from the loop below)
+    const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), wm = wave / WN, wn = wave % WN;
+    int tm, tn;
+    place(p, split ? p.whole + t : unit, tm, tn);
+    const int first = step0 * BK, end = min(p.k, step1 * BK);
+    const int direct = DIRECT ? (end - first) / BK : 0, steps = (end - first + BK - 1) / BK;
+    LA la{(const T *)p.a, p.lda, tm * BM, p.m, p.k, wave, lane};
+    LB lb{(const T *)p.b, p.ldb, tn * BN, p.n, p.k, wave, lane};
+    f4 acc[MI][NI] = {};
+    typedef typename Half<T>::frag frag;
+    const auto read = [&](const char *ta, int ks, frag (&a)[MI], frag (&b)[NI]) {
 #pragma unroll
-    for (int j = 0; j < NI; j++) b[j] = TB::template fragment<T>(ta + TA::kBytes, wn * (BN / WN) + j * 16, ks, lane);
+      for (int j = 0; j < NI; j++) b[j] = TB::template fragment<T>(ta + TA::kBytes, wn * (BN / WN) + j * 16, ks, lane);
 #pragma unroll
-    for (int i = 0; i < MI; i++) a[i] = TA::template fragment<T>(ta, wm * (BM / WM) + i * 16, ks, lane);
-  };
-  const auto multiply = [&](const frag (&a)[MI], const frag (&b)[NI]) {
+      for (int i = 0; i < MI; i++) a[i] = TA::template fragment<T>(ta, wm * (BM / WM) + i * 16, ks, lane);
+    };
+    const auto multiply = [&](const frag (&a)[MI], const frag (&b)[NI]) {
 #pragma unroll
-    for (int i = 0; i < MI; i++)
+      for (int i = 0; i < MI; i++)
 #pragma unroll
-      for (int j = 0; j < NI; j++) Half<T>::mfma(b[j], a[i], acc[i][j]);      // (n, m): a lane ends with 4 consecutive n of one m
-  };
-  // the order of a half: its loads and LDS reads spread over the first part of its matrix instructions
-  constexpr int READS = (A_ACROSS ? 2 : 1) * MI + (B_ACROSS ? 2 : 1) * NI;
-  const auto interleave = [&](auto loads) {
-    constexpr int L = decltype(loads)::value, PER = MI * NI / (READS + L) > 0 ? MI * NI / (READS + L) : 1;
+        for (int j = 0; j < NI; j++) Half<T>::mfma(b[j], a[i], acc[i][j]);      // (n, m): a lane ends with 4 consecutive n of one m
+    };
+    // the order of a half: its loads and LDS reads spread over the first part of its matrix instructions
+    constexpr int READS = (A_ACROSS ? 2 : 1) * MI + (B_ACROSS ? 2 : 1) * NI;
+    const auto interleave = [&](auto loads) {
+      constexpr int L = decltype(loads)::value, PER = MI * NI / (READS + L) > 0 ? MI * NI / (READS + L) : 1;
 #pragma unroll
-    for (int i = 0; i < READS; i++) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
-    }
+      for (int i = 0; i < READS; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+      }
 #pragma unroll
-    for (int i = 0; i < L; i++) {
-      __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, MI * NI, 0);
-  };
-  if constexpr (DIRECT) {
-    if (direct) {
-      const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char *)lds;
-      la.start(first);
-      lb.start(first);
-      unsigned load = 0;      // where the next tile goes
-      const auto issue = [&](int) {
-        la.direct(lds0 + load);
-        lb.direct(lds0 + load + TA::kBytes);
-        load = load == (STAGES - 1) * kStage ? 0 : load + kStage;
-      };
-      issue(0);
-      if constexpr (PIPED) {
-        frag a0[MI], b0[NI], a1[MI], b1[NI];
-        __syncthreads();
-        if (direct > 1) issue(1);
-        read(lds, 0, a0, b0);
-        const auto step = [&](int s, auto loads) {
-          read(lds + (s & 1) * kStage, 1, a1, b1);
-          multiply(a0, b0);
-          interleave(std::integral_constant<int, 0>());
-          arrive<0>();
-          if constexpr (decltype(loads)::value) issue(s);
-          read(lds + ((s & 1) ^ 1) * kStage, 0, a0, b0);      // (behind the last tile: something from LDS, for nothing)
-          multiply(a1, b1);
-          interleave(loads);
+      for (int i = 0; i < L; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, MI * NI, 0);
+    };
+    if constexpr (DIRECT) {
+      if (direct) {
+        const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char *)lds;
+        la.start(first);
+        lb.start(first);
+        unsigned load = 0;      // where the next tile goes
+        const auto issue = [&](int) {
+          la.direct(lds0 + load);
+          lb.direct(lds0 + load + TA::kBytes);
+          load = load == (STAGES - 1) * kStage ? 0 : load + kStage;
         };
-        int s = 0;
-        for (; s + 2 < direct; s++) step(s, std::integral_constant<int, LA::N + LB::N>());
-        for (; s < direct; s++) step(s, std::integral_constant<int, 0>());
-      } else {
-        // STAGES - 1 tiles are on their way while one is multiplied
+        issue(0);
+        if constexpr (PIPED) {
+          frag a0[MI], b0[NI], a1[MI], b1[NI];
+          __syncthreads();
+          if (direct > 1) issue(1);
+          read(lds, 0, a0, b0);
+          const auto step = [&](int s, auto loads) {
+            read(lds + (s & 1) * kStage, 1, a1, b1);
+            multiply(a0, b0);
+            interleave(std::integral_constant<int, 0>());
+            arrive<0>();
+            if constexpr (decltype(loads)::value) issue(s);
+            read(lds + ((s & 1) ^ 1) * kStage, 0, a0, b0);      // (behind the last tile: something from LDS, for nothing)
+            multiply(a1, b1);
+            interleave(loads);
+          };
+          int s = 0;
+          for (; s + 2 < direct; s++) step(s, std::integral_constant<int, LA::N + LB::N>());
+          for (; s < direct; s++) step(s, std::integral_constant<int, 0>());
+        } else {
+          // STAGES - 1 tiles are on their way while one is multiplied
 #pragma unroll
-        for (int i = 1; i < STAGES - 1; i++) if (i < direct) issue(i);
-        unsigned now = 0;
-        for (int s = 0; s < direct; s++) {
-          if (s + STAGES - 2 < direct) arrive<(STAGES - 2) * (LA::N + LB::N)>();
-          else arrive<0>();
-          if (s + STAGES - 1 < direct) issue(s + STAGES - 1);
+          for (int i = 1; i < STAGES - 1; i++) if (i < direct) issue(i);
+          unsigned now = 0;
+          for (int s = 0; s < direct; s++) {
+            if (s + STAGES - 2 < direct) arrive<(STAGES - 2) * (LA::N + LB::N)>();
+            else arrive<0>();
+            if (s + STAGES - 1 < direct) issue(s + STAGES - 1);
+            frag a[MI], b[NI];
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+              read(lds + now, ks, a, b);
+              multiply(a, b);
+            }
+            now = now == (STAGES - 1) * kStage ? 0 : now + kStage;
+          }
+        }
+        __syncthreads();
+      }
+    }
+    // what is left of the contraction (everything, where the operands' alignment does not allow the direct way): through registers, R tiles of them on their way
+    if (direct < steps) {
+      constexpr int R = DIRECT || BM >= 128 ? 1 : 3;      // (two of 128 x 128 would leave a compute unit one workgroup instead of two)
+      typename LA::chunk va[R][LA::N];
+      typename LB::chunk vb[R][LB::N];
+      la.fetch(first + direct * BK, va[0]);
+      lb.fetch(first + direct * BK, vb[0]);
+      la.store(lds, va[0]);
+      lb.store(lds + TA::kBytes, vb[0]);
+#pragma unroll
+      for (int r = 0; r < R; r++)
+        if (direct + 1 + r < steps) {
+          la.fetch(first + (direct + 1 + r) * BK, va[r]);
+          lb.fetch(first + (direct + 1 + r) * BK, vb[r]);
+        }
+      __syncthreads();
+      for (int s0 = direct; s0 < steps; s0 += R)
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          const int s = s0 + r, now = (s - direct) & 1;
+          if (s >= steps) break;
           frag a[MI], b[NI];
 #pragma unroll
           for (int ks = 0; ks < 2; ks++) {
-            read(lds + now, ks, a, b);
+            read(lds + now * kStage, ks, a, b);
             multiply(a, b);
           }
-          now = now == (STAGES - 1) * kStage ? 0 : now + kStage;
-        }
-      }
-      __syncthreads();
-    }
-  }
-  // what is left of the contraction (everything, where the operands' alignment does not allow the direct way): through registers, R tiles of them on their way
-  if (direct < steps) {
-    constexpr int R = DIRECT || BM >= 128 ? 1 : 3;      // (two of 128 x 128 would leave a compute unit one workgroup instead of two)
-    typename LA::chunk va[R][LA::N];
-    typename LB::chunk vb[R][LB::N];
-    la.fetch(first + direct * BK, va[0]);
-    lb.fetch(first + direct * BK, vb[0]);
-    la.store(lds, va[0]);
-    lb.store(lds + TA::kBytes, vb[0]);
-#pragma unroll
-    for (int r = 0; r < R; r++)
-      if (direct + 1 + r < steps) {
-        la.fetch(first + (direct + 1 + r) * BK, va[r]);
-        lb.fetch(first + (direct + 1 + r) * BK, vb[r]);
-      }
-    __syncthreads();
-    for (int s0 = direct; s0 < steps; s0 += R)
-#pragma unroll
-      for (int r = 0; r < R; r++) {
-        const int s = s0 + r, now = (s - direct) & 1;
-        if (s >= steps) break;
-        frag a[MI], b[NI];
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++) {
-          read(lds + now * kStage, ks, a, b);
-          multiply(a, b);
-        }
-        if (s + 1 < steps) {
-          la.store(lds + (now ^ 1) * kStage, va[r]);
-          lb.store(lds + (now ^ 1) * kStage + TA::kBytes, vb[r]);
-          if (s + 1 + R < steps) {
-            la.fetch(first + (s + 1 + R) * BK, va[r]);
-            lb.fetch(first + (s + 1 + R) * BK, vb[r]);
+          if (s + 1 < steps) {
+            la.store(lds + (now ^ 1) * kStage, va[r]);
+            lb.store(lds + (now ^ 1) * kStage + TA::kBytes, vb[r]);
+            if (s + 1 + R < steps) {
+              la.fetch(first + (s + 1 + R) * BK, va[r]);
+              lb.fetch(first + (s + 1 + R) * BK, vb[r]);
+            }
           }
+          __syncthreads();
         }
-        __syncthreads();
-      }
-  }
-  // The epilogue goes through LDS, a part of each wavefront's rows at a time (as many as its share of the tiles' memory holds): out of the accumulators' layout (4 columns of one of 16 rows
-  // per lane) into runs of whole rows, so that what is read and written beside it are lines.  A row's chunk c of 4 lies at c ^ a function of the row that differs among the 16 rows that are
-  // written at once.
-  constexpr int CW = BN / WN, Q = CW / 4, SHARE = (int)sizeof(lds) / (WM * WN) / 16 * 16, HOLD = SHARE / (CW * 4) / 16 * 16;
-  constexpr int PASS = HOLD >= BM / WM ? BM / WM : BM / WM / 2, STRIDE = 64 / (Q / 2), U = PASS / STRIDE;      // rows per pass, rows between a lane's, and rows per lane
-  static_assert(PASS >= 16 && PASS <= HOLD && (BM / WM) % PASS == 0 && U >= 1, "rows per pass");
-  f4 *mine = (f4 *)(lds + wave * SHARE);
-  const int m0 = tm * BM + wm * (BM / WM), n0 = tn * BN + wn * CW;
-  float *sums = p.partial + (long long)(unit + t) * (BM * BN) + wm * (BM / WM) * BN + wn * CW;
+    }
+    // The epilogue goes through LDS, a part of each wavefront's rows at a time (as many as its share of the tiles' memory holds): out of the accumulators' layout (4 columns of one of 16 rows
+    // per lane) into runs of whole rows, so that what is read and written beside it are lines.  A row's chunk c of 4 lies at c ^ a function of the row that differs among the 16 rows that are
+    // written at once.
+    constexpr int CW = BN / WN, Q = CW / 4, SHARE = (int)sizeof(lds) / (WM * WN) / 16 * 16, HOLD = SHARE / (CW * 4) / 16 * 16;
+    constexpr int PASS = HOLD >= BM / WM ? BM / WM : BM / WM / 2, STRIDE = 64 / (Q / 2), U = PASS / STRIDE;      // rows per pass, rows between a lane's, and rows per lane
+    static_assert(PASS >= 16 && PASS <= HOLD && (BM / WM) % PASS == 0 && U >= 1, "rows per pass");
+    f4 *mine = (f4 *)(lds + wave * SHARE);
+    const int m0 = tm * BM + wm * (BM / WM), n0 = tn * BN + wn * CW;
+    float *sums = p.partial + (long long)(unit + t) * (BM * BN) + wm * (BM / WM) * BN + wn * CW;
 #pragma unroll
-  for (int i0 = 0; i0 < MI; i0 += PASS / 16) {
+    for (int i0 = 0; i0 < MI; i0 += PASS / 16) {
 #pragma unroll
-    for (int i = 0; i < PASS / 16; i++)
+      for (int i = 0; i < PASS / 16; i++)
 #pragma unroll
-      for (int j = 0; j < NI; j++) {
-        const int r = i * 16 + (lane & 15), c = j * 4 + (lane >> 4);
-        mine[r * Q + (c ^ (r / (16 / Q) & (Q - 1)))] = acc[i0 + i][j];
-      }
-    wave_fence();
-    const int r0 = lane / (Q / 2), c = lane % (Q / 2) * 2;      // this lane's first row and columns of the pass
-    const auto value = [&](int u) {
-      const int r = r0 + u * STRIDE, f = r / (16 / Q) & (Q - 1);
-      return __builtin_shufflevector(mine[r * Q + (c ^ f)], mine[r * Q + ((c + 1) ^ f)], 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    if (piece) {
+        for (int j = 0; j < NI; j++) {
+          const int r = i * 16 + (lane & 15), c = j * 4 + (lane >> 4);
+          mine[r * Q + (c ^ (r / (16 / Q) & (Q - 1)))] = acc[i0 + i][j];
+        }
+      wave_fence();
+      const int r0 = lane / (Q / 2), c = lane % (Q / 2) * 2;      // this lane's first row and columns of the pass
+      const auto value = [&](int u) {
+        const int r = r0 + u * STRIDE, f = r / (16 / Q) & (Q - 1);
+        return __builtin_shufflevector(mine[r * Q + (c ^ f)], mine[r * Q + ((c + 1) ^ f)], 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+      if (piece) {
 #pragma unroll 1
-      for (int u = 0; u < U; u++) *(f8 *)(sums + (i0 * 16 + r0 + u * STRIDE) * BN + c * 4) = value(u);
-    } else if (n0 + CW <= p.n && p.e.act <= kRelu) finish_rows<T, U>(p.e, m0 + i0 * 16 + r0, STRIDE, p.m, n0 + c * 4, value);
-    else
+        for (int u = 0; u < U; u++) *(f8 *)(sums + (i0 * 16 + r0 + u * STRIDE) * BN + c * 4) = value(u);
+      } else if (n0 + CW <= p.n && p.e.act <= kRelu) finish_rows<T, U>(p.e, m0 + i0 * 16 + r0, STRIDE, p.m, n0 + c * 4, value);
+      else
 #pragma unroll 1
-      for (int u = 0; u < U; u++) {
-        const long long row = m0 + i0 * 16 + r0 + u * STRIDE;
-        if (row < p.m && n0 + c * 4 < p.n) finish<T>(p.e, row, n0 + c * 4, p.n - n0 - c * 4, value(u));
-      }
-    wave_fence();
-  }
-  if (split) __syncthreads();      // (LDS is the next piece's)
+        for (int u = 0; u < U; u++) {
+          const long long row = m0 + i0 * 16 + r0 + u * STRIDE;
+          if (row < p.m && n0 + c * 4 < p.n) finish<T>(p.e, row, n0 + c * 4, p.n - n0 - c * 4, value(u));
+        }
+      wave_fence();
+    }
+    if (split) __syncthreads();      // (LDS is the next piece's)
   } while (at < run_end);
 }
 

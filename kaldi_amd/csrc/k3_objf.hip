@@ -6,7 +6,7 @@
 // overflow at the lowest values of float32 and bfloat16, which masks are made of.
 // Bound by memory, a row being read once (and its derivative written once): scores of float32 42752 x 6024 with 4 alternatives 168 us (6.1 TB/s), label derivative of bfloat16 2000 x 50001
 // 78 us (5.1), distillation with derivative of float32 6400 x 6024 67 us (4.6) and of bfloat16 4096 x 128000 508 us (4.1: a row fills a compute unit's registers, and its
-// vector instructions, 54 % of the cycles by counters, run under its own loads and stores only in part).
+// vector instructions, 53 to 55 % of its cycles by counters, run under its own loads and stores only in part).
 #include "k3_rowops.h"
 #include <algorithm>
 #include <type_traits>
@@ -660,7 +660,12 @@ extern "C" int k3_label_logprobs_deriv(int32_t dtype, const void *d_z, int64_t l
   K3_REQUIRE(rows >= 0 && cols >= 1 && ld >= cols && ldd >= cols, "k3_label_logprobs_deriv: bad argument");
   if (rows == 0) return K3_OK;
   K3_REQUIRE(d_z && d_dz && d_stats && (d_labels || !d_log_prob_deriv) && (d_entropy || !d_entropy_deriv), "k3_label_logprobs_deriv: null input");
-#define K3_LABEL_DERIV(T)                                                                                                                                                       const int segments = (cols + 256 * Chunk<T>::N - 1) / (256 * Chunk<T>::N);                                                                                                    const long long items = (long long)rows * segments, blocks = (items + 3) / 4;                                                                                                 K3_REQUIRE(blocks < (1ll << 31), "k3_label_logprobs_deriv: matrix too large");                                                                                                hipLaunchKernelGGL((k3_label_deriv_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const T *)d_z, (long long)ld, d_labels, d_stats, d_entropy,                             d_log_prob_deriv, d_entropy_deriv, (T *)d_dz, (long long)ldd, cols, segments, items)
+#define K3_LABEL_DERIV(T)                                                                                                                            \
+  const int segments = (cols + 256 * Chunk<T>::N - 1) / (256 * Chunk<T>::N);                                                                         \
+  const long long items = (long long)rows * segments, blocks = (items + 3) / 4;                                                                      \
+  K3_REQUIRE(blocks < (1ll << 31), "k3_label_logprobs_deriv: matrix too large");                                                                     \
+  hipLaunchKernelGGL((k3_label_deriv_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const T *)d_z, (long long)ld, d_labels, \
+                    d_stats, d_entropy, d_log_prob_deriv, d_entropy_deriv, (T *)d_dz, (long long)ldd, cols, segments, items)
   K3_FOR_DTYPE(dtype, K3_LABEL_DERIV);
   K3_HIP_CHECK(hipGetLastError());
   return K3_OK;
