@@ -300,7 +300,8 @@ __device__ inline void join_parts(const Partial *part, int splits, float a, floa
   Partial q = {-kInf, 0.0f, 0.0f, 0.0f};
   if (lane < splits) q = part[lane];
   m = wave_max(q.max);
-  const float d = q.max == -kInf ? 0.0f : (q.max - m) * a, f = exp2_fast(d);      // (a part without values has s = u = 0, or NaN)
+  // (a part without values has s = u = 0, or NaN.  One of nothing but the type's lowest value is so far below the row's largest that d overflows: at -16384 its f is 0 all the same, and f d too)
+  const float d = q.max == -kInf ? 0.0f : fmaxf((q.max - m) * a, -16384.0f), f = exp2_fast(d);
   s = wave_sum(q.sum * f);
   u = wave_sum(q.weighted * f + q.sum * f * d);
 }

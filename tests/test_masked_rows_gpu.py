@@ -1,0 +1,34 @@
+"""GPU tests of the label scores and of distillation on rows of which a range of columns holds the type's lowest value, as masks do that are added or filled in (kaldi_amd.objective), against
+the formulas in float64.
+
+Bounds: those of the tests with ordinary values, S(n, D) = (n / 64 + 2 D + 40) half steps of float32, with D = 40 (a column further below the row's largest adds less than 2^-57 of the
+sum, masked ones nothing)."""
+import pytest, torch
+from tests.rowop_cases import TYPES, U32, half_step, empty_like, untouched, assert_within, generator
+pytestmark = pytest.mark.gpu
+
+def S(n, D=40): return (n / 64 + 2 * D + 40) * U32
+def tiny(dtype): return 2.0 ** -25 if dtype == torch.float16 else 1e-30
+
+def masked_rows(cols, dtype):
+    """rows with a masked head, tail, middle, everything but the first or the last column, every third range of 2048 columns, everything, and nothing; the rest is of unit size"""
+    z = torch.randn(8, cols, generator=generator(cols), device="cuda").to(dtype); low = torch.finfo(dtype).min; c = torch.arange(cols, device="cuda"); third = cols // 3
+    for r, m in enumerate((c < third, c >= cols - third, (c >= third) & (c < 2 * third), c > 0, c < cols - 1, c // 2048 % 3 == 1, c >= 0)): z[r] = torch.where(m, torch.full_like(z[r], low), z[r])
+    return z
+
+# one part per row; parts of few rows (2048 columns and more); parts that a workgroup holds of float32, of halves; the most columns
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [300, 4096, 9001, 16385, 40000, 70001, 131073, 1 << 19])
+def test_scores_and_their_derivative(cols, dtype):
+    from kaldi_amd.objective import LabelLogProbs, DiffLabelLogProbs
+    z = masked_rows(cols, dtype); n = z.shape[0]; y = torch.tensor([cols - 1, 0, cols // 2, 0, cols - 1, 1, 7, -1], dtype=torch.int32, device="cuda"); y[2] = 0
+    lp, h, st = torch.empty(n, device="cuda"), torch.empty(n, device="cuda"), torch.empty(n, 2, device="cuda"); LabelLogProbs(z, y, lp, h, st)
+    # (the largest value is taken away first: beside the lowest number even float64 has no room for a logarithm)
+    m = z.double().amax(1); x = z.double() - m[:, None]; ls = torch.logsumexp(x, 1); lq = x - ls[:, None]; q = lq.exp(); H = -torch.where(q > 0, q * lq, 0.0).sum(1); err = S(cols) + 4 * U32 * ls.abs()
+    assert torch.equal(st[:, 0].double(), m); assert_within(st[:, 1], ls, err, "log sum")
+    want = torch.where(y >= 0, lq.gather(1, y.long().clamp(min=0)[:, None])[:, 0], 0.0); assert_within(lp, want, err + 3 * U32 * want.abs(), "log prob")
+    assert_within(h, H, err + (S(cols) + 8 * U32) * (H + ls), "entropy")
+    a, b = torch.randn(n, generator=generator(1), device="cuda"), torch.randn(n, generator=generator(2), device="cuda"); dz = empty_like(z); DiffLabelLogProbs(z, y, st, h, a, b, dz); assert untouched(dz)
+    ga, gb = torch.where(y >= 0, a, 0.0).double()[:, None], b.double()[:, None]; inner = lq.clamp(min=-1e4) + H[:, None]; want = -q * (ga + gb * inner); want[torch.arange(n, device="cuda"), y.long().clamp(min=0)] += ga[:, 0]
+    e = S(cols) + 4 * U32 * (ls[:, None].abs() + 101.0); off = q * (e + 4 * U32) * (ga.abs() + gb.abs() * (inner.abs() + H[:, None] + ls[:, None].abs() + 2)) + 4 * U32 * want.abs() + 2 * U32 * ga.abs() * (want.abs() > 0)
+    assert_within(dz, want, half_step(dtype) * (want.abs() + off) + off + tiny(dtype), "dz")
