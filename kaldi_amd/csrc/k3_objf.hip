@@ -369,7 +369,7 @@ struct DistillArgs {
   float *objf; void *dz; long long ldd;
   int splits; const Partial *partial; float4 *coef; float *prob;      // of the rows that are too wide for one workgroup
 };
-// a row's teacher entries in LDS: column (-1: not used), the teacher's e and d, and the student's value there
+// a row's teacher entries in LDS: column (-1: not used), the teacher's e and value below its largest, and the student's value there
 struct Entry { int col; float e, d, z; };
 struct Teacher { float sum; bool live; };      // sum of the e; whether the row counts (an entry that is not -inf, and a weight that is not 0)
 
@@ -391,7 +391,7 @@ template <typename T, int NW> __device__ inline Teacher teacher_softmax(const Di
   float s = 0.0f;
   for (int k = t; k < p.top; k += 64 * NW) {
     const int c = entry[k].col;
-    const float v = entry[k].d, d = v == -kInf ? -kInf : (v - m) * p.a, e = exp2_fast(d);
+    const float v = entry[k].d, d = v == -kInf ? -kInf : v - m, e = exp2_fast(d * p.a);
     entry[k].z = c >= 0 ? to_f32(((const T *)p.z)[row * p.ld + c]) : 0.0f;
     entry[k].d = d;
     entry[k].e = e;
@@ -399,13 +399,15 @@ template <typename T, int NW> __device__ inline Teacher teacher_softmax(const Di
   }
   return Teacher{block_sum<NW>(s, sh + NW), m != -kInf && !(p.weights && p.weights[row] == 0.0f)};
 }
-// sum_k p_k (log q_k - log p_k) from the student's M and s; in every thread
+// T sum_k p_k (log q_k - log p_k) from the student's M and s; in every thread.  Differences stay in the logits' units and are divided by the teacher's sum (at least 1) one by one: in those
+// of the exponentials, or summed before the division, one with a lowest value in it would overflow, which the objective does not
 template <int NW> __device__ inline float teacher_objf(const DistillArgs &p, const Entry *entry, Teacher w, float m, float s, int t, float *sh) {
   float f = 0.0f;
+  const float r = 1.0f / w.sum;
   for (int k = t; k < p.top; k += 64 * NW)
-    if (!(entry[k].e == 0.0f)) f += entry[k].e * ((entry[k].z - m) * p.a - entry[k].d);
-  f = block_sum<NW>(f, sh) / w.sum;
-  return m == -kInf && s == s ? -kInf : kLn2 * (f + (log2f(w.sum) - log2f(s)));
+    if (!(entry[k].e == 0.0f)) f += entry[k].e * (r * (entry[k].z - m - entry[k].d));
+  f = block_sum<NW>(f, sh);
+  return m == -kInf && s == s ? -kInf : f + p.temperature * kLn2 * (log2f(w.sum) - log2f(s));
 }
 
 // One row per NW wavefronts, held in registers from the sums to the derivative: read once, written once.  The teacher's columns are corrected behind the row's own store (by the same
@@ -442,7 +444,7 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
   if (empty) m = -kInf;
   const float w = (p.weights ? p.weights[row] : 1.0f) * p.temperature;
   const float f = teacher_objf<NW>(p, entry, teacher, m, s, t, sh + 4 * NW);
-  if (t == 0) p.objf[row] = teacher.live ? w * p.temperature * f : 0.0f;
+  if (t == 0) p.objf[row] = teacher.live ? w * f : 0.0f;
   if (!p.dz) return;
   T *dz = (T *)p.dz + row * p.ldd;
   if (!teacher.live || empty) {
@@ -473,7 +475,7 @@ template <typename T> __global__ __launch_bounds__(64) void k3_distill_join_kern
   join_parts(p.partial + row * p.splits, p.splits, p.a, m, s, u);
   const float w = (p.weights ? p.weights[row] : 1.0f) * p.temperature, f = teacher_objf<1>(p, entries, teacher, m, s, t, nullptr);
   if (t == 0) {
-    p.objf[row] = teacher.live ? w * p.temperature * f : 0.0f;
+    p.objf[row] = teacher.live ? w * f : 0.0f;
     if (p.dz) p.coef[row] = make_float4(m, -w / s, w, teacher.live && !(m == -kInf && s == s) ? 1.0f : 0.0f);
   }
   if (p.dz)

@@ -32,3 +32,25 @@ def test_scores_and_their_derivative(cols, dtype):
     ga, gb = torch.where(y >= 0, a, 0.0).double()[:, None], b.double()[:, None]; inner = lq.clamp(min=-1e4) + H[:, None]; want = -q * (ga + gb * inner); want[torch.arange(n, device="cuda"), y.long().clamp(min=0)] += ga[:, 0]
     e = S(cols) + 4 * U32 * (ls[:, None].abs() + 101.0); off = q * (e + 4 * U32) * (ga.abs() + gb.abs() * (inner.abs() + H[:, None] + ls[:, None].abs() + 2)) + 4 * U32 * want.abs() + 2 * U32 * ga.abs() * (want.abs() > 0)
     assert_within(dz, want, half_step(dtype) * (want.abs() + off) + off + tiny(dtype), "dz")
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [300, 4096, 9001, 70001, 140001])
+def test_distillation_with_entries_at_masked_columns(cols, dtype):
+    """the objective there is w T p (z - M), within the range of float32 for the probabilities chosen, though not (z - M) / T for T < 1.44.  The differences are off by a few half steps
+    of their sizes, which S covers as it does for ordinary ones"""
+    from kaldi_amd.objective import ComputeDistillObjfAndDeriv, DistillationOptions
+    z = masked_rows(cols, dtype); n, c = z.shape[0], cols // 2; g = generator(cols + 1); third = cols // 3
+    # columns in every range: most of each row's entries are at masked ones in some row, with probabilities of a tenth or less; the teacher has a masked entry of its own
+    idx = torch.tensor([[0, c, cols - 1, 1, c + 1, cols - 2, third, -1]], dtype=torch.int32, device="cuda").repeat(n, 1); idx[7, 0] = 5
+    t = torch.tensor([[4.0, 1.0, 0.5, 0.2, 0.1, float(torch.finfo(dtype).min), 0.3, 9.0]], device="cuda").to(dtype).repeat(n, 1); order = torch.tensor([2, 0, 0, 0, 2, 0, 1, 0])
+    for r in range(n): k = int(order[r]); t[r, [0, k]] = t[r, [k, 0]]
+    w = torch.tensor([1.0, 0.5, -0.25, 1.0, 0.5, 1.0, 1.0, 2.0], device="cuda"); f, dz, alone = torch.empty(n, device="cuda"), empty_like(z), torch.empty(n, device="cuda")
+    for T in (0.5, 1.0, 1.4, 2.0):
+        o = DistillationOptions(T); ComputeDistillObjfAndDeriv(o, z, t, idx, w, f, dz); ComputeDistillObjfAndDeriv(o, z, t, idx, w, alone); assert untouched(dz)
+        used = idx >= 0; at = idx.long().clamp(min=0); tt = torch.where(used, t.double(), -float("inf")) / T; tt = tt - tt.amax(1, keepdim=True); lp = tt - torch.logsumexp(tt, 1, keepdim=True); p = torch.where(used, lp.exp(), 0.0)
+        x = (z.double() - z.double().amax(1, keepdim=True)) / T; lq = x - torch.logsumexp(x, 1, keepdim=True); lqk = lq.gather(1, at); D = 40.0 + 8.0 / T; e = S(cols, D) + S(64, D)
+        want = w.double() * T * T * torch.where(p > 0, p * (lqk - lp), 0.0).sum(1); mag = w.double().abs() * T * T * torch.where(p > 0, p * (lqk.abs() + lp.abs() + 1), 0.0).sum(1); assert (want.abs() < 3.4e38).all()
+        if dtype != torch.float16: assert (want.abs() > 1e30).sum() >= 4      # (masked columns do count: ordinary ones give less than 100)
+        assert_within(f, want, e * mag, "objf"); assert_within(alone, want, e * mag, "objf alone")
+        P = torch.zeros_like(lq).scatter_add_(1, at, p); d = w.double()[:, None] * T * (P - lq.exp()); off = e * w.double().abs()[:, None] * T * (P + lq.exp())
+        assert_within(dz, d, half_step(dtype) * (d.abs() + off) + off + tiny(dtype), "dz")
