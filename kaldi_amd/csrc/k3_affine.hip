@@ -44,9 +44,10 @@ __device__ inline float slope(int act, float z) {
   z = z < -1e4f ? -1e4f : z > 1e4f ? 1e4f : z;
   switch (act) {
     case kRelu: return z > 0.0f ? 1.0f : z == z ? 0.0f : z;
-    case kSigmoid: { const float s = sigmoid(z); return s * (1.0f - s); }
-    case kTanh: { const float s = tanh_fast(z); return 1.0f - s * s; }
-    case kSwish: { const float s = sigmoid(z); return s * (1.0f + z * (1.0f - s)); }
+    // (from t = e^-|z|, sigmoid(|z|) = 1 / (1 + t) and sigmoid(-|z|) = t / (1 + t): 1 - sigmoid(z) would cancel where z is large)
+    case kSigmoid: { const float t = exp_fast(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + t); return t * r * r; }
+    case kTanh: { const float t = exp_fast(-2.0f * fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + t); return 4.0f * t * r * r; }
+    case kSwish: { const float t = exp_fast(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + t), s = z < 0.0f ? t * r : r, c = z < 0.0f ? r : t * r; return s * (1.0f + z * c); }
     case kGelu: { float e; const float f = erf_half(z, e); return 0.5f * (1.0f + f) + z * 0.39894228040143268f * e; }
     default: return 1.0f;
   }
