@@ -22,12 +22,14 @@ __device__ inline float tanh_fast(float z) {
   const float q = z * z;
   return fabsf(z) < 0.1f ? z * (1.0f + q * (-0.33333333f + q * 0.13333333f)) : 1.0f - 2.0f * __builtin_amdgcn_rcpf(exp_fast(2.0f * z) + 1.0f);
 }
-// erf(z / sqrt 2) to 1.5e-7 (Abramowitz and Stegun, 7.1.26), with e = exp(-z^2 / 2) for who needs it too
-__device__ inline float erf_half(float z, float &e) {
-  const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+// 1 + erf(z / sqrt 2), with e = exp(-z^2 / 2) for who needs it too.  erfc(x) e^(x^2) = t P(t), t = 1 / (1 + 0.4 x), to a relative 1.3e-7 for all x >= 0 (P fitted in float64 to
+// the smallest largest relative error): for z < 0 the result is erfc itself, which 1 - (1 - erfc) would leave no digits of
+__device__ inline float one_plus_erf(float z, float &e) {
+  const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.0f + 0.4f * x);
   e = exp_fast(-0.5f * z * z);
-  const float r = 1.0f - t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * e;
-  return z < 0.0f ? -r : r;
+  const float c = e * t * (0.225675866f + t * (0.225669608f + t * (0.207842514f + t * (0.168543801f + t * (0.141422957f + t * (-0.00558652263f +
+                  t * (0.169057027f + t * (-0.182881743f + t * 0.0502566323f))))))));
+  return z < 0.0f ? c : 2.0f - c;
 }
 // (-inf goes in as a number whose exponential is 0 all the same: 0 times it is 0)
 __device__ inline float activation(int act, float z) {
@@ -36,7 +38,7 @@ __device__ inline float activation(int act, float z) {
     case kSigmoid: return sigmoid(z);
     case kTanh: return tanh_fast(z);
     case kSwish: z = z < -1e4f ? -1e4f : z; return z * sigmoid(z);
-    case kGelu: { float e; z = z < -1e4f ? -1e4f : z; return 0.5f * z * (1.0f + erf_half(z, e)); }
+    case kGelu: { float e; z = z < -1e4f ? -1e4f : z; return 0.5f * z * one_plus_erf(z, e); }
     default: return z;
   }
 }
@@ -48,7 +50,7 @@ __device__ inline float slope(int act, float z) {
     case kSigmoid: { const float t = exp_fast(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + t); return t * r * r; }
     case kTanh: { const float t = exp_fast(-2.0f * fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + t); return 4.0f * t * r * r; }
     case kSwish: { const float t = exp_fast(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + t), s = z < 0.0f ? t * r : r, c = z < 0.0f ? r : t * r; return s * (1.0f + z * c); }
-    case kGelu: { float e; const float f = erf_half(z, e); return 0.5f * (1.0f + f) + z * 0.39894228040143268f * e; }
+    case kGelu: { float e; const float f = one_plus_erf(z, e); return 0.5f * f + z * 0.39894228040143268f * e; }
     default: return 1.0f;
   }
 }

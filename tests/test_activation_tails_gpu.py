@@ -33,3 +33,15 @@ def slopes(act, dtype):
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("act", ["sigmoid", "tanh", "swish"])
 def test_slopes_in_the_tails(act, dtype): slopes(act, dtype)
+
+@pytest.mark.parametrize("dtype", HALVES)
+def test_gelus_slope_in_the_tails(dtype): slopes("gelu", dtype)
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("act", ["sigmoid", "tanh", "swish", "gelu"])
+def test_values_in_the_tails(act, dtype):
+    """tanh between -0.1 and 0.1 is a series, beside it a difference from 1 that is off by 2 half steps of 1"""
+    from kaldi_amd.cumatrix import AffinePerRow
+    z = points(dtype); y = torch.empty(z.numel(), 1, dtype=dtype, device="cuda"); AffinePerRow(z[:, None], torch.ones(1, 1, device="cuda").to(dtype), None, act, None, y)
+    want = act64(act, z.double()); off = relative(act, z.double()) * want.abs() + (4 * U32 if act == "tanh" else 0.0) + 2.0 ** -119
+    assert_within(y[:, 0], want, half_step(dtype) * (want.abs() + off) + off + SMALLEST[dtype], "value")
