@@ -17,6 +17,13 @@ using namespace k3;
 // as a rule, for half-precision values) stays.
 __device__ inline float left_mean(float m0, float d, float q) { return m0 * m0 > 64.0f * q ? d : 0.0f; }
 
+// 1 / sqrt(var + eps) from the mean square q of the differences from m0 and what m0 is off by.  (Not below 0 by rounding; a NaN, of a row that holds NaNs or infinities, stays one, as fmaxf
+// would not let it.)
+__device__ inline float inv_std_of(float q, float d, float eps) {
+  const float var = q - d * d;
+  return 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
+}
+
 // The rows a launch can hold in registers (up to 1024 threads of 16 or 24 elements).  A row belongs to NW wavefronts (one: four rows per workgroup); thread t holds the chunks t, t + 64 NW,
 // ... of it, E of them, so each element is read once and both sums of the forward pass run over registers.  A workgroup walks over rows with a stride of the whole launch: scale
 // and offset stay in registers, and the next row is on its way while this one is reduced and written.
@@ -64,7 +71,7 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
     }
     block_sum2<NW>(d, q, sh + NW);
     d = left_mean(m0, d / n, q / n);
-    const float r = 1.0f / sqrtf(fmaxf(q / n - d * d, 0.0f) + eps), m1 = m0 + d;
+    const float r = inv_std_of(q / n, d, eps), m1 = m0 + d;
     if (t == 0) {
       if (mean) mean[row] = m1;
       if (inv_std) inv_std[row] = r;
@@ -200,7 +207,7 @@ template <typename T> __global__ __launch_bounds__(256) void k3_ln_forward_loop_
   for (int c = threadIdx.x; c < cols; c += 256) { const float v = to_f32(xr[c]) - m0; d += v; q += v * v; }
   block_sum2<4>(d, q, sh + 4);
   d = left_mean(m0, d / (float)cols, q / (float)cols);
-  const float r = 1.0f / sqrtf(fmaxf(q / (float)cols - d * d, 0.0f) + eps);
+  const float r = inv_std_of(q / (float)cols, d, eps);
   if (threadIdx.x == 0) {
     if (mean) mean[row] = m0 + d;
     if (inv_std) inv_std[row] = r;
