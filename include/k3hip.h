@@ -566,12 +566,12 @@ int k3_chain_objf_and_deriv(k3_chain_den *den, k3_chain_supervision *sup, const 
 typedef enum { K3_F32 = 0, K3_F16 = 1, K3_BF16 = 2 } k3_dtype;
 /* Layer norm of every row: y = (x - mean) inv_std scale + offset with inv_std = 1 / sqrt(var + eps), var = the mean square of x - mean.  Stands beside cu::NormalizePerRow
  * (cudamatrix/cu-math.h:272), which takes no mean away.  d_scale / d_offset [cols] may be null (1 / 0); d_mean / d_inv_std [rows] (null: not kept) are what the backward pass takes.
- * y may be x.  cols = 0 or rows = 0: nothing to do. */
+ * y may be x.  cols = 0 or rows = 0: nothing to do.  At most 2^31 - 1024 columns. */
 int k3_layer_norm_forward(int32_t dtype, const void *d_x, int64_t ldx, const float *d_scale, const float *d_offset, float eps, void *d_y, int64_t ldy,
                           float *d_mean, float *d_inv_std, int32_t rows, int32_t cols, void *stream);
 /* Its derivatives from dy: d_dx (null: not wanted; may be dy or x), d_dscale / d_doffset [cols] (null: not wanted), overwritten, or added to with accumulate != 0 (rows = 0 then leaves
  * them; otherwise it clears them).  Sums over rows are taken in a fixed order: the same call gives the same bits.  d_workspace: k3_layer_norm_backward_workspace(rows, cols) bytes,
- * 16-byte aligned, needed only where d_dscale or d_doffset is wanted. */
+ * 16-byte aligned, needed only where d_dscale or d_doffset is wanted.  At most 2^31 - 1024 columns, 2^28 - 64 where d_dscale or d_doffset is wanted. */
 int64_t k3_layer_norm_backward_workspace(int32_t rows, int32_t cols);
 int k3_layer_norm_backward(int32_t dtype, const void *d_x, int64_t ldx, const void *d_dy, int64_t lddy, const float *d_scale, const float *d_mean, const float *d_inv_std,
                            void *d_dx, int64_t lddx, float *d_dscale, float *d_doffset, int32_t accumulate, void *d_workspace, int64_t workspace_bytes,

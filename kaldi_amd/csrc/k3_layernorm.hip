@@ -279,6 +279,8 @@ __global__ __launch_bounds__(1024) void k3_ln_param_join_kernel(const float *par
 }
 
 const int kMaxStrips = 512;
+const int kMaxCols = 0x7fffffff - 1023;      // column numbers of threads that run ahead of a row's end still fit 32 bits
+const int kMaxParamCols = (1 << 28) - 64;    // k3_ln_param_join_kernel has 16 threads per column, and a launch less than 2^32
 
 // wavefronts per row and chunks per thread: the fewest wavefronts that hold the row with at most 16 (float) or 24 elements per thread, and no more than 16 of them (then 12 or 16
 // elements: a workgroup of 1024 has 128 registers per thread, and one chunk more spills in the backward pass); {0, 0} = too wide
@@ -348,6 +350,7 @@ extern "C" int k3_layer_norm_forward(int32_t dtype, const void *d_x, int64_t ldx
                                      float *d_mean, float *d_inv_std, int32_t rows, int32_t cols, void *stream) {
   K3_REQUIRE(dtype_ok(dtype), "k3_layer_norm_forward: unknown type");
   K3_REQUIRE(rows >= 0 && cols >= 0 && ldx >= cols && ldy >= cols && eps >= 0.0f, "k3_layer_norm_forward: bad argument");
+  if (cols > kMaxCols) { set_error("k3_layer_norm_forward: at most %d columns", kMaxCols); return K3_ERR_UNSUPPORTED; }
   if (rows == 0 || cols == 0) return K3_OK;
   K3_REQUIRE(d_x && d_y, "k3_layer_norm_forward: null matrix");
 #define K3_LN_FWD(T) forward<T>(d_x, ldx, d_scale, d_offset, eps, d_y, ldy, d_mean, d_inv_std, rows, cols, (hipStream_t)stream)
@@ -366,9 +369,13 @@ extern "C" int k3_layer_norm_backward(int32_t dtype, const void *d_x, int64_t ld
                                       int32_t rows, int32_t cols, void *stream) {
   K3_REQUIRE(dtype_ok(dtype), "k3_layer_norm_backward: unknown type");
   K3_REQUIRE(rows >= 0 && cols >= 0 && ldx >= cols && lddy >= cols && (!d_dx || lddx >= cols), "k3_layer_norm_backward: bad argument");
+  const bool params = d_dscale || d_doffset;
+  if (cols > (params ? kMaxParamCols : kMaxCols)) {
+    set_error("k3_layer_norm_backward: at most %d columns, with the derivatives of scale or offset %d", kMaxCols, kMaxParamCols);
+    return K3_ERR_UNSUPPORTED;
+  }
   if (cols == 0) return K3_OK;
   K3_REQUIRE(rows == 0 || (d_x && d_dy && d_mean && d_inv_std), "k3_layer_norm_backward: null input");
-  const bool params = d_dscale || d_doffset;
   K3_REQUIRE(!params || rows == 0 || (d_workspace && workspace_bytes >= k3_layer_norm_backward_workspace(rows, cols)), "k3_layer_norm_backward: workspace too small");
   hipStream_t st = (hipStream_t)stream;
   int strips = 0;
