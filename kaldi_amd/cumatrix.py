@@ -21,6 +21,7 @@ def _rows(m, name):
     t = m.t if type(m) is CuMatrix else m
     try: dt = _DTYPES[t.dtype]; r, c = t.shape; s0, s1 = t.stride(); i = t.get_device()
     except (AttributeError, KeyError, ValueError, RuntimeError): _refuse(f"{name}: a matrix of float32, float16 or bfloat16 is wanted")
+    if r > 0x7fffffff or c > 0x7fffffff: _refuse(f"{name}: {r} x {c}: at most 2^31 - 1 rows and columns")      # (the C entries' sizes are int32, and ctypes would cut them)
     if i < 0: _refuse(f"{name}: not on a GPU")
     if r <= 1: s0 = c
     if (s1 != 1 and c > 1) or s0 < c: _refuse(f"{name}: rows must be contiguous and must not overlap (strides {s0}, {s1})")

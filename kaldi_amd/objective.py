@@ -11,6 +11,7 @@ def LabelLogProbs(nnet_output, labels, log_prob=None, entropy=None, stats=None, 
     dt, z, ld, r, c, i = _rows(nnet_output, "nnet_output")
     alt = alt_log_probs if alt_log_probs is not None else alt_labels
     n = 0 if alt is None else alt.shape[-1]
+    if n > 64: _refuse(f"alternatives: {n}, at most 64 are kept")
     L = _l.load(); nw = L.k3_label_logprobs_workspace(dt, r, c, n); w = _workspace(nw, i)
     _run(i, L.k3_label_logprobs, dt, z, ld, _vec(labels, r, i, "labels", _I32), _vec(log_prob, r, i, "log_prob"), _vec(entropy, r, i, "entropy"), _table(stats, r, 2, i, "stats"), n,
          _table(alt_log_probs, r, n, i, "alt_log_probs"), _table(alt_labels, r, n, i, "alt_labels", _I32), w.data_ptr() if nw else None, nw, r, c)

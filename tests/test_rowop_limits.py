@@ -11,3 +11,13 @@ def test_layer_norm_of_rows_whose_column_numbers_pass_32_bits():
     assert fwd(most) == 0 and bwd(most) == 0      # (without rows: nothing is queued)
     for cols in ((1 << 28) - 63, 1 << 30, most): refused(bwd(cols, P), "at most"); refused(bwd(cols, None, P), "at most")
     refused(bwd((1 << 28) - 64, P), "workspace")      # (gets as far as that)
+
+def test_sizes_that_do_not_fit_32_bits():
+    """on tensors without memory: what does not fit is refused before where they are is looked at"""
+    from kaldi_amd import cumatrix as cm, objective as ob
+    from kaldi_amd.lib import K3Error
+    for shape in ((1 << 31, 1), ((1 << 32) + 4, 8), (1, 1 << 31), (4, (1 << 32) + 8)):
+        t = torch.empty(shape, dtype=torch.float16, device="meta")
+        for call in (lambda: cm.LayerNormPerRow(t, None, None, 1e-5, t), lambda: cm.AffinePerRow(t, t, None, "none", None, t), lambda: cm.DiffAffinePerRow(t, t, None, "none", t), lambda: ob.LabelLogProbs(t, None),
+                     lambda: cm.DiffLayerNormPerRow(t, t, None, None, None), lambda: ob.DiffLabelLogProbs(t, None, None, None, None, None, t), lambda: ob.ComputeDistillObjfAndDeriv(ob.DistillationOptions(), t, t, t, None, None)):
+            with pytest.raises(K3Error, match="2\\^31"): call()
