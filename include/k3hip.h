@@ -562,7 +562,8 @@ int k3_chain_objf_and_deriv(k3_chain_den *den, k3_chain_supervision *sup, const 
  * Operators for training and scoring around a network's output.  Matrices are row-major with a leading dimension (elements; >= cols, no alignment asked of it or of the pointers
  * beyond the element's own) of one of the types below; vectors and statistics are float32 unless said otherwise.  Sums are kept in float32 and a result is rounded once, when
  * it is written.  A call queues its kernels on `stream` of the current device and returns; nothing is allocated, copied to the host or waited for, so calls can be captured into
- * graphs.  Where a workspace is asked for, it holds nothing between calls: two calls may share one only if the stream (or the graph) runs them one after the other. */
+ * graphs.  A matrix or vector that a call writes shares no element with its other operands, unless it is said to be allowed: then it is that operand, leading dimension included
+ * (columns of one buffer side by side share none).  Where a workspace is asked for, it holds nothing between calls: two calls may share one only if the stream (or the graph) runs them one after the other. */
 typedef enum { K3_F32 = 0, K3_F16 = 1, K3_BF16 = 2 } k3_dtype;
 /* Layer norm of every row: y = (x - mean) inv_std scale + offset with inv_std = 1 / sqrt(var + eps), var = the mean square of x - mean.  Stands beside cu::NormalizePerRow
  * (cudamatrix/cu-math.h:272), which takes no mean away.  d_scale / d_offset [cols] may be null (1 / 0); d_mean / d_inv_std [rows] (null: not kept) are what the backward pass takes.
@@ -577,14 +578,14 @@ int k3_layer_norm_backward(int32_t dtype, const void *d_x, int64_t ldx, const vo
                            void *d_dx, int64_t lddx, float *d_dscale, float *d_doffset, int32_t accumulate, void *d_workspace, int64_t workspace_bytes,
                            int32_t rows, int32_t cols, void *stream);
 /* An affine layer in half precision (dtype K3_F16 or K3_BF16): pre = x W^T + bias, y = act(pre) + residual, x [rows x inner], W [cols x inner] (AffineComponent's linear_params),
- * d_bias float32 [cols] (null: 0), d_residual [rows x cols] (null: none; y may be it, and no other matrix).  d_pre (null: not kept) receives pre as the backward pass takes it.  Products are summed in float32 and
+ * d_bias float32 [cols] (null: 0), d_residual [rows x cols] (null: none; y may be it).  d_pre (null: not kept) receives pre as the backward pass takes it.  Products are summed in float32 and
  * a result is rounded once.  Stands beside k3_mat_add_mat_mat, which is float32 and has no epilogue.  Workspace (16-byte aligned): k3_affine_forward_workspace. */
 typedef enum { K3_ACT_NONE = 0, K3_ACT_RELU = 1, K3_ACT_SIGMOID = 2, K3_ACT_TANH = 3, K3_ACT_SWISH = 4 /* z sigmoid(z) */, K3_ACT_GELU = 5 /* z (1 + erf(z / sqrt 2)) / 2 */ } k3_activation;
 int64_t k3_affine_forward_workspace(int32_t rows, int32_t inner, int32_t cols);
 int k3_affine_forward(int32_t dtype, int32_t act, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const float *d_bias, const void *d_residual, int64_t ldr, void *d_y,
                       int64_t ldy, void *d_pre, int64_t ldp, void *d_workspace, int64_t workspace_bytes, int32_t rows, int32_t inner, int32_t cols, void *stream);
 /* Its derivatives from dy: dz = dy act'(pre) (d_pre not read for K3_ACT_NONE), d_dx = dz W and d_dw = dz^T x (of the matrices' type), d_db [cols] = the sum of dz over the rows (float32);
- * each may be null (not wanted), and what is given is overwritten and lies on no input.  (The residual's derivative is dy itself.)  Where there is an activation, dz is rounded to the matrices' type for the two
+ * each may be null (not wanted), and what is given is overwritten.  (The residual's derivative is dy itself.)  Where there is an activation, dz is rounded to the matrices' type for the two
  * products, not for d_db.  Sums are taken in a fixed order.  rows = 0 clears d_dw and d_db.  Workspace (16-byte aligned): k3_affine_backward_workspace. */
 int64_t k3_affine_backward_workspace(int32_t act, int32_t rows, int32_t inner, int32_t cols);
 int k3_affine_backward(int32_t dtype, int32_t act, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_pre, int64_t ldp, const void *d_dy, int64_t lddy,

@@ -653,7 +653,9 @@ extern "C" int k3_affine_forward(int32_t dtype, int32_t act, const void *d_x, in
   if (!sizes_ok(rows, inner, cols)) { set_error("k3_affine_forward: matrix too large"); return K3_ERR_UNSUPPORTED; }
   if (rows == 0) return K3_OK;
   K3_REQUIRE(d_x && d_w && d_y, "k3_affine_forward: null matrix");
-  K3_REQUIRE(d_y != d_x && d_y != d_w && d_y != d_pre && (!d_pre || (d_pre != d_x && d_pre != d_w && d_pre != d_residual)), "k3_affine_forward: an output lies on another matrix");
+  const Span x = matrix_span(d_x, ldx, rows, inner, 2), w = matrix_span(d_w, ldw, cols, inner, 2), b = vector_span(d_bias, cols), r = matrix_span(d_residual, ldr, rows, cols, 2),
+             y = matrix_span(d_y, ldy, rows, cols, 2), pre = matrix_span(d_pre, ldp, rows, cols, 2);
+  K3_REQUIRE(!on_any(y, {x, w, b, pre}) && !on_any(pre, {x, w, b, r}) && (same(y, r) || !overlap(y, r)), "k3_affine_forward: an output lies on another matrix");
   K3_REQUIRE(workspace_bytes >= k3_affine_forward_workspace(rows, inner, cols) && (d_workspace || workspace_bytes == 0) && ((uintptr_t)d_workspace & 15) == 0,
              "k3_affine_forward: workspace too small or not aligned");
   Product p{};
@@ -677,11 +679,13 @@ extern "C" int k3_affine_backward(int32_t dtype, int32_t act, const void *d_x, i
              "k3_affine_backward: bad argument");
   if (!sizes_ok(rows, inner, cols)) { set_error("k3_affine_backward: matrix too large"); return K3_ERR_UNSUPPORTED; }
   K3_REQUIRE(rows == 0 || (d_dy && (d_x || !d_dw) && (d_w || !d_dx) && (d_pre || act == kNone)), "k3_affine_backward: null input");
-  for (const void *out : {(const void *)d_dx, (const void *)d_dw})
-    K3_REQUIRE(!out || rows == 0 || (out != d_x && out != d_w && out != d_dy && (act == kNone || out != d_pre)), "k3_affine_backward: an output lies on an input");
-  K3_REQUIRE(!d_dx || d_dx != d_dw, "k3_affine_backward: the outputs lie on each other");
+  const Span x = matrix_span(ldx >= inner ? d_x : nullptr, ldx, rows, inner, 2), w = matrix_span(ldw >= inner ? d_w : nullptr, ldw, cols, inner, 2), dy = matrix_span(d_dy, lddy, rows, cols, 2),
+             pre = matrix_span(act == kNone ? nullptr : d_pre, ldp, rows, cols, 2), dx = matrix_span(d_dx, lddx, rows, inner, 2), dw = matrix_span(d_dw, lddw, cols, inner, 2), db = vector_span(d_db, cols);
+  K3_REQUIRE(rows == 0 || (!on_any(dx, {x, w, dy, pre}) && !on_any(dw, {x, w, dy, pre})), "k3_affine_backward: an output lies on an input");
+  K3_REQUIRE(!overlap(dx, dw) && !on_any(db, {dx, dw}), "k3_affine_backward: the outputs lie on each other");
   K3_REQUIRE(workspace_bytes >= k3_affine_backward_workspace(act, rows, inner, cols) && (d_workspace || workspace_bytes == 0) && ((uintptr_t)d_workspace & 15) == 0,
              "k3_affine_backward: workspace too small or not aligned");
+  K3_REQUIRE(rows == 0 || !on_any(db, {x, w, dy, pre}), "k3_affine_backward: an output lies on an input");
   const Backward q{d_x, ldx, d_w, ldw, d_pre, ldp, d_dy, lddy, rows ? d_dx : nullptr, lddx, d_dw, lddw, d_db, act, rows, inner, cols};
   return dtype == K3_F16 ? affine_backward<f16>(q, (char *)d_workspace, (hipStream_t)stream) : affine_backward<bf16>(q, (char *)d_workspace, (hipStream_t)stream);
 }

@@ -136,6 +136,35 @@ template <int NW> __device__ inline void block_sum2(float &a, float &b, float *s
 inline bool dtype_ok(int dtype) { return dtype >= K3_F32 && dtype <= K3_BF16; }
 inline size_t dtype_size(int dtype) { return dtype == K3_F32 ? 4 : 2; }
 
+// ---- which memory an operand takes: a call that writes a matrix where another of its operands lies is refused, since workgroups read and write in no order
+struct Span {      // `rows` pieces of `width` bytes, `stride` apart (at least `width` where there are several); none: p null, or rows or width 0
+  uintptr_t p; int64_t stride, rows, width;
+  uintptr_t end() const { return p + (rows - 1) * stride + width; }
+  bool none() const { return !p || rows <= 0 || width <= 0; }
+};
+inline Span matrix_span(const void *p, int64_t ld, int64_t rows, int64_t cols, size_t size) { return {(uintptr_t)p, ld * (int64_t)size, rows, cols * (int64_t)size}; }
+inline Span vector_span(const void *p, int64_t n, size_t size = 4) { return {(uintptr_t)p, n * (int64_t)size, 1, n * (int64_t)size}; }
+// the same elements at the same places
+inline bool same(const Span &a, const Span &b) { return a.p == b.p && a.rows == b.rows && a.width == b.width && (a.rows <= 1 || a.stride == b.stride); }
+inline bool overlap(const Span &a, const Span &b) {
+  if (a.none() || b.none() || a.end() <= b.p || b.end() <= a.p) return false;
+  if (a.rows > 1 && b.rows > 1 && a.stride == b.stride) {      // columns of one buffer, side by side or not
+    const int64_t d = (int64_t)(b.p - a.p) % a.stride, at = d < 0 ? d + a.stride : d;
+    return at < a.width || at + b.width > a.stride;
+  }
+  const Span &f = a.rows <= b.rows ? a : b, &m = a.rows <= b.rows ? b : a;
+  for (int64_t i = 0; i < f.rows; i++) {      // the first piece of the other that ends behind this one's start: does it start before this one's end
+    const uintptr_t s = f.p + i * f.stride, e = s + f.width;
+    const int64_t j = s < m.p + m.width ? 0 : (int64_t)((s - m.p - m.width) / m.stride) + 1;
+    if (j < m.rows && m.p + j * m.stride < e) return true;
+  }
+  return false;
+}
+template <size_t N> inline bool on_any(const Span &out, const Span (&others)[N]) {
+  for (const Span &o : others) if (overlap(out, o)) return true;
+  return false;
+}
+
 }  // namespace k3
 
 // f(T{}) for the type of a k3_dtype that has been checked

@@ -1,0 +1,19 @@
+"""Operands that share memory: which calls of the operators on rows of matrices refuse it (on the host, with addresses that are never used; no GPU is needed for those)."""
+import torch
+from kaldi_amd import lib as _l
+from tests.test_rowop_refusals import P, refused
+
+def test_affine_layer():
+    L = _l.load(); R, K, C = 6, 40, 24; n = L.k3_affine_forward_workspace(R, K, C)
+    f = lambda x=P, ldx=K, w=2 * P, ldw=K, b=3 * P, r=4 * P, ldr=C, y=5 * P, ldy=C, pre=6 * P, ldp=C, rows=R: L.k3_affine_forward(1, 1, x, ldx, w, ldw, b, r, ldr, y, ldy, pre, ldp, 9 * P, n, rows, K, C, None)  # noqa: E731
+    end = 2 * ((R - 1) * K + K)      # of x
+    for at in (P + 2, P + 2 * K, P + end - 2, P - 2 * ((R - 1) * C + C) + 2): refused(f(y=at), "lies on"); refused(f(pre=at), "lies on")
+    for at in (2 * P + 2, 2 * P + 2 * C * K - 2, 3 * P, 3 * P + 4 * C - 2): refused(f(y=at), "lies on"); refused(f(pre=at), "lies on")      # the weights, the bias
+    refused(f(y=4 * P, ldy=C + 1), "lies on"); refused(f(y=4 * P, ldr=C + 8), "lies on"); refused(f(y=4 * P + 2), "lies on"); refused(f(y=4 * P + 2 * C), "lies on"); refused(f(pre=4 * P), "lies on")      # the residual, but for its own place
+    refused(f(y=5 * P, pre=5 * P + 2 * C * R - 2), "lies on")
+    refused(f(ldx=100, ldy=100, y=P + 2 * (K - 1)), "lies on"); refused(f(ldx=100, ldy=100, y=P + 2 * (100 - C + 1)), "lies on")      # columns of one buffer that reach into each other, in one row or the next
+    refused(f(ldx=100, ldy=90, y=P + 2 * K), "lies on"); refused(f(rows=2, ldx=100, ldy=50, y=P + 2 * 60), "lies on")                 # strides that differ: the second row meets x
+    n = L.k3_affine_backward_workspace(1, R, K, C)
+    b = lambda x=P, ldx=K, w=2 * P, pre=3 * P, dy=4 * P, lddy=C, dx=5 * P, lddx=K, dw=6 * P, lddw=K, db=7 * P: L.k3_affine_backward(1, 1, x, ldx, w, K, pre, C, dy, lddy, dx, lddx, dw, lddw, db, 9 * P, n, R, K, C, None)  # noqa: E731
+    for at in (P + 2, P + end - 2, 2 * P + 2 * C * K - 2, 3 * P + 2 * C * R - 2, 4 * P + 2): refused(b(dx=at), "lies on"); refused(b(dw=at), "lies on"); refused(b(db=at), "lies on")
+    refused(b(dx=4 * P + 2 * (C - 1), lddy=100, lddx=100), "lies on"); refused(b(dw=5 * P + end - 2), "lie on each other"); refused(b(db=5 * P + 4), "lie on each other"); refused(b(db=6 * P), "lie on each other")

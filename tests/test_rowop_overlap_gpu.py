@@ -1,0 +1,31 @@
+"""GPU tests of the operators on rows of matrices with operands that share a buffer without sharing an element of it: results are those of operands of their own."""
+import torch, pytest
+from tests.rowop_cases import generator
+pytestmark = pytest.mark.gpu
+
+def beside(*shapes, dtype, gap=0):
+    """matrices of equal numbers of rows as columns of one buffer, `gap` elements apart"""
+    base = torch.full((shapes[0][0], sum(c + gap for _, c in shapes)), 77.0, dtype=dtype, device="cuda"); at = 0; out = []
+    for _, c in shapes: out.append(base[:, at:at + c]); at += c + gap
+    return out
+
+def test_affine_layer_within_one_buffer():
+    from kaldi_amd.cumatrix import AffinePerRow, DiffAffinePerRow
+    for dtype in (torch.float16, torch.bfloat16):
+        for R, K, C, gap in ((300, 64, 136, 0), (37, 41, 19, 3), (1, 64, 8, 0)):
+            g = generator(R); x, y, pre, r, dx, dy = beside((R, K), (R, C), (R, C), (R, C), (R, K), (R, C), dtype=dtype, gap=gap); w = torch.randn(C, K, generator=g, device="cuda").to(dtype); b = torch.randn(C, generator=g, device="cuda")
+            for t in (x, r, dy): t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+            own = [t.clone() for t in (x, r, dy)]; y2, pre2, dx2 = (torch.empty_like(t.contiguous()) for t in (y, pre, dx)); AffinePerRow(x, w, b, "gelu", r, y, pre); AffinePerRow(own[0], w, b, "gelu", own[1], y2, pre2)
+            assert torch.equal(y, y2) and torch.equal(pre, pre2)
+            dw, db, dw2, db2 = torch.empty_like(w), torch.empty_like(b), torch.empty_like(w), torch.empty_like(b); DiffAffinePerRow(x, w, pre, "gelu", dy, dx, dw, db); DiffAffinePerRow(own[0], w, pre2, "gelu", own[2], dx2, dw2, db2)
+            assert torch.equal(dx, dx2) and torch.equal(dw, dw2) and torch.equal(db, db2) and all(torch.equal(p, q) for p, q in zip((x, r, dy), own))
+            # every second row of a buffer, and rows in front of each other
+            rows = torch.empty(2 * R, C, dtype=dtype, device="cuda"); rows[::2] = r; AffinePerRow(x, w, b, "gelu", rows[::2], rows[1::2]); assert torch.equal(rows[1::2], y2) and torch.equal(rows[::2], own[1])
+            rows = torch.empty(2 * R, C, dtype=dtype, device="cuda"); rows[R:] = r; AffinePerRow(x, w, b, "gelu", rows[R:], rows[:R]); assert torch.equal(rows[:R], y2)
+            AffinePerRow(x, w, b, "gelu", r, r); assert torch.equal(r, y2)
+
+def test_affine_layer_in_the_gaps_of_another_stride():
+    """a matrix of two wide rows, and the other one's rows of another stride between and behind them"""
+    from kaldi_amd.cumatrix import AffinePerRow
+    g = generator(1); base = torch.full((400,), 77.0, dtype=torch.float16, device="cuda"); x = base.as_strided((2, 40), (200, 1), 0); y = base.as_strided((2, 24), (220, 1), 50); x.copy_(torch.randn(2, 40, generator=g, device="cuda")); w = torch.randn(24, 40, generator=g, device="cuda").half()
+    own, want = x.contiguous(), torch.empty(2, 24, dtype=torch.float16, device="cuda"); AffinePerRow(own, w, None, "none", None, want); AffinePerRow(x, w, None, "none", None, y); assert torch.equal(y, want) and torch.equal(x, own)
