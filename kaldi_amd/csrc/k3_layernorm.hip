@@ -353,6 +353,10 @@ extern "C" int k3_layer_norm_forward(int32_t dtype, const void *d_x, int64_t ldx
   if (cols > kMaxCols) { set_error("k3_layer_norm_forward: at most %d columns", kMaxCols); return K3_ERR_UNSUPPORTED; }
   if (rows == 0 || cols == 0) return K3_OK;
   K3_REQUIRE(d_x && d_y, "k3_layer_norm_forward: null matrix");
+  const size_t size = dtype_size(dtype);
+  const Span x = matrix_span(d_x, ldx, rows, cols, size), y = matrix_span(d_y, ldy, rows, cols, size), sc = vector_span(d_scale, cols), of = vector_span(d_offset, cols),
+             mean = vector_span(d_mean, rows), inv = vector_span(d_inv_std, rows);
+  K3_REQUIRE((same(x, y) || !overlap(x, y)) && !on_any(y, {sc, of, mean, inv}) && !on_any(mean, {x, sc, of}) && !on_any(inv, {x, sc, of}), "k3_layer_norm_forward: an output lies on another operand");
 #define K3_LN_FWD(T) forward<T>(d_x, ldx, d_scale, d_offset, eps, d_y, ldy, d_mean, d_inv_std, rows, cols, (hipStream_t)stream)
   K3_FOR_DTYPE(dtype, K3_LN_FWD);
   K3_HIP_CHECK(hipGetLastError());
@@ -377,6 +381,11 @@ extern "C" int k3_layer_norm_backward(int32_t dtype, const void *d_x, int64_t ld
   if (cols == 0) return K3_OK;
   K3_REQUIRE(rows == 0 || (d_x && d_dy && d_mean && d_inv_std), "k3_layer_norm_backward: null input");
   K3_REQUIRE(!params || rows == 0 || (d_workspace && workspace_bytes >= k3_layer_norm_backward_workspace(rows, cols)), "k3_layer_norm_backward: workspace too small");
+  // (d_dscale and d_doffset are written when everything else has been read)
+  const size_t size = dtype_size(dtype);
+  const Span x = matrix_span(d_x, ldx, rows, cols, size), dy = matrix_span(d_dy, lddy, rows, cols, size), dx = matrix_span(d_dx, lddx, rows, cols, size), sc = vector_span(d_scale, cols),
+             mean = vector_span(d_mean, rows), inv = vector_span(d_inv_std, rows), ds = vector_span(d_dscale, cols), doff = vector_span(d_doffset, cols);
+  K3_REQUIRE((same(x, dx) || !overlap(x, dx)) && (same(dy, dx) || !overlap(dy, dx)) && !on_any(dx, {sc, mean, inv, ds, doff}) && !overlap(ds, doff), "k3_layer_norm_backward: an output lies on another operand");
   hipStream_t st = (hipStream_t)stream;
   int strips = 0;
   if (rows && (params || d_dx)) {

@@ -17,3 +17,16 @@ def test_affine_layer():
     b = lambda x=P, ldx=K, w=2 * P, pre=3 * P, dy=4 * P, lddy=C, dx=5 * P, lddx=K, dw=6 * P, lddw=K, db=7 * P: L.k3_affine_backward(1, 1, x, ldx, w, K, pre, C, dy, lddy, dx, lddx, dw, lddw, db, 9 * P, n, R, K, C, None)  # noqa: E731
     for at in (P + 2, P + end - 2, 2 * P + 2 * C * K - 2, 3 * P + 2 * C * R - 2, 4 * P + 2): refused(b(dx=at), "lies on"); refused(b(dw=at), "lies on"); refused(b(db=at), "lies on")
     refused(b(dx=4 * P + 2 * (C - 1), lddy=100, lddx=100), "lies on"); refused(b(dw=5 * P + end - 2), "lie on each other"); refused(b(db=5 * P + 4), "lie on each other"); refused(b(db=6 * P), "lie on each other")
+
+def test_layer_norm():
+    L = _l.load(); R, C, X = 6, 40, 4
+    for dtype, size in ((0, 4), (1, 2), (2, 2)):
+        f = lambda x=P, ldx=C, sc=2 * P, of=3 * P, y=5 * P, ldy=C, m=6 * P, i=7 * P: L.k3_layer_norm_forward(dtype, x, ldx, sc, of, 1e-5, y, ldy, m, i, R, C, None)  # noqa: E731
+        for at in (P + size, P + size * (R * C - 1), 2 * P, 3 * P + 4 * C - size, 6 * P, 7 * P + 4 * R - size): refused(f(y=at), "lies on")
+        for k in ("m", "i"):
+            for at in (P, P + size * R * C - 4, 2 * P + 4, 3 * P): refused(f(**{k: at}), "lies on")
+        refused(f(y=P, ldy=C + 1), "lies on"); refused(f(y=P, ldx=C + 8), "lies on"); refused(f(ldx=100, ldy=100, y=P + size * (C - 1)), "lies on"); refused(f(ldx=100, ldy=100, y=P - size * (C - 1)), "lies on")
+        n = L.k3_layer_norm_backward_workspace(R, C)
+        b = lambda x=P, ldx=C, dy=2 * P, lddy=C, sc=3 * P, m=4 * P, i=5 * P, dx=6 * P, lddx=C, ds=7 * P, do=8 * P: L.k3_layer_norm_backward(dtype, x, ldx, dy, lddy, sc, m, i, dx, lddx, ds, do, 0, 9 * P, n, R, C, None)  # noqa: E731
+        for at in (P + size, 2 * P + size, P + size * (R * C - 1), 2 * P - size, 3 * P, 4 * P, 5 * P + 4 * R - size, 7 * P, 8 * P + 4 * C - size): refused(b(dx=at), "lies on")
+        for k in (dict(dx=P, lddx=C + 1), dict(dx=2 * P, lddx=C + 8), dict(dx=P, ldx=C + 1), dict(dx=2 * P, lddy=C + 1), dict(ds=8 * P), dict(do=7 * P + 4 * C - 4)): refused(b(**k), "lies on")

@@ -29,3 +29,14 @@ def test_affine_layer_in_the_gaps_of_another_stride():
     from kaldi_amd.cumatrix import AffinePerRow
     g = generator(1); base = torch.full((400,), 77.0, dtype=torch.float16, device="cuda"); x = base.as_strided((2, 40), (200, 1), 0); y = base.as_strided((2, 24), (220, 1), 50); x.copy_(torch.randn(2, 40, generator=g, device="cuda")); w = torch.randn(24, 40, generator=g, device="cuda").half()
     own, want = x.contiguous(), torch.empty(2, 24, dtype=torch.float16, device="cuda"); AffinePerRow(own, w, None, "none", None, want); AffinePerRow(x, w, None, "none", None, y); assert torch.equal(y, want) and torch.equal(x, own)
+
+def test_layer_norm_within_one_buffer():
+    from kaldi_amd.cumatrix import LayerNormPerRow, DiffLayerNormPerRow
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        for R, C, gap in ((50, 136, 0), (37, 19, 3), (1, 64, 0), (9, 20011, 1)):
+            g = generator(C); x, y, dy, dx = beside((R, C), (R, C), (R, C), (R, C), dtype=dtype, gap=gap); x.copy_(torch.randn(R, C, generator=g, device="cuda")); dy.copy_(torch.randn(R, C, generator=g, device="cuda")); stats = torch.empty(2, R, device="cuda"); vectors = torch.randn(4, C, generator=g, device="cuda")
+            ox, ody, oy, odx = x.clone(), dy.clone(), torch.empty_like(x.contiguous()), torch.empty_like(x.contiguous()); om, oi, ods, odo = torch.empty(R, device="cuda"), torch.empty(R, device="cuda"), torch.empty(C, device="cuda"), torch.empty(C, device="cuda")
+            LayerNormPerRow(ox, vectors[0].clone(), vectors[1].clone(), 1e-5, oy, om, oi); DiffLayerNormPerRow(ox, ody, vectors[0].clone(), om, oi, odx, ods, odo)
+            LayerNormPerRow(x, vectors[0], vectors[1], 1e-5, y, stats[0], stats[1]); DiffLayerNormPerRow(x, dy, vectors[0], stats[0], stats[1], dx, vectors[2], vectors[3])      # the vectors are neighbours too
+            assert torch.equal(y, oy) and torch.equal(stats[0], om) and torch.equal(stats[1], oi) and torch.equal(dx, odx) and torch.equal(vectors[2], ods) and torch.equal(vectors[3], odo) and torch.equal(x, ox) and torch.equal(dy, ody)
+            DiffLayerNormPerRow(x, dy, vectors[0], stats[0], stats[1], dy); assert torch.equal(dy, odx); LayerNormPerRow(x, vectors[0], vectors[1], 1e-5, x); assert torch.equal(x, oy)
