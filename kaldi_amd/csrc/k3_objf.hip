@@ -648,6 +648,10 @@ extern "C" int k3_label_logprobs(int32_t dtype, const void *d_z, int64_t ld, con
   K3_REQUIRE(d_z && (d_labels || !d_log_prob), "k3_label_logprobs: null input");
   const int64_t need = k3_label_logprobs_workspace(dtype, rows, cols, num_alternatives);
   K3_REQUIRE(need == 0 || (d_workspace && workspace_bytes >= need && ((uintptr_t)d_workspace & 15) == 0), "k3_label_logprobs: workspace too small or not aligned");
+  const Span z = matrix_span(d_z, ld, rows, cols, dtype_size(dtype)), y = vector_span(d_labels, rows);
+  for (const Span &out : {vector_span(d_log_prob, rows), vector_span(d_entropy, rows), vector_span(d_stats, 2 * (int64_t)rows), vector_span(d_alt_log_probs, (int64_t)rows * num_alternatives),
+                          vector_span(d_alt_labels, (int64_t)rows * num_alternatives)})
+    K3_REQUIRE(!on_any(out, {z, y}), "k3_label_logprobs: an output lies on an input");
   ScoreArgs p{};
   p.z = d_z; p.ld = ld; p.rows = rows; p.cols = cols; p.labels = d_labels; p.a = kLog2e;
   p.log_prob = d_log_prob; p.entropy = d_entropy; p.stats = d_stats; p.alt_log_probs = d_alt_log_probs; p.alt_labels = d_alt_labels; p.top = num_alternatives;
@@ -663,6 +667,9 @@ extern "C" int k3_label_logprobs_deriv(int32_t dtype, const void *d_z, int64_t l
   K3_REQUIRE(rows >= 0 && cols >= 1 && ld >= cols && ldd >= cols, "k3_label_logprobs_deriv: bad argument");
   if (rows == 0) return K3_OK;
   K3_REQUIRE(d_z && d_dz && d_stats && (d_labels || !d_log_prob_deriv) && (d_entropy || !d_entropy_deriv), "k3_label_logprobs_deriv: null input");
+  const Span z = matrix_span(d_z, ld, rows, cols, dtype_size(dtype)), dz = matrix_span(d_dz, ldd, rows, cols, dtype_size(dtype));
+  K3_REQUIRE((same(z, dz) || !overlap(z, dz)) && !on_any(dz, {vector_span(d_labels, rows), vector_span(d_stats, 2 * (int64_t)rows), vector_span(d_entropy, rows), vector_span(d_log_prob_deriv, rows),
+                                                              vector_span(d_entropy_deriv, rows)}), "k3_label_logprobs_deriv: the output lies on another operand");
 #define K3_LABEL_DERIV(T)                                                                                                                            \
   const int segments = (cols + 256 * Chunk<T>::N - 1) / (256 * Chunk<T>::N);                                                                         \
   const long long items = (long long)rows * segments, blocks = (items + 3) / 4;                                                                      \
@@ -691,6 +698,10 @@ extern "C" int k3_distill_objf_and_deriv(int32_t dtype, float temperature, const
   K3_REQUIRE(d_z && d_teacher_values && d_teacher_indexes && d_objf, "k3_distill_objf_and_deriv: null input");
   const int64_t need = k3_distill_workspace(dtype, rows, cols, num_entries, d_dz != nullptr);
   K3_REQUIRE(need == 0 || (d_workspace && workspace_bytes >= need && ((uintptr_t)d_workspace & 15) == 0), "k3_distill_objf_and_deriv: workspace too small or not aligned");
+  const size_t size = dtype_size(dtype);
+  const Span z = matrix_span(d_z, ld, rows, cols, size), v = matrix_span(d_teacher_values, ld_values, rows, num_entries, size), i = matrix_span(d_teacher_indexes, ld_indexes, rows, num_entries, 4),
+             w = vector_span(d_weights, rows), f = vector_span(d_objf, rows), dz = matrix_span(d_dz, ldd, rows, cols, size);
+  K3_REQUIRE((same(z, dz) || !overlap(z, dz)) && !on_any(dz, {v, i, w, f}) && !on_any(f, {z, v, i, w}), "k3_distill_objf_and_deriv: an output lies on another operand");
   DistillArgs p{};
   p.z = d_z; p.ld = ld; p.rows = rows; p.cols = cols; p.values = d_teacher_values; p.ld_values = ld_values; p.indexes = d_teacher_indexes; p.ld_indexes = ld_indexes;
   p.top = num_entries; p.weights = d_weights; p.temperature = temperature; p.a = kLog2e / temperature; p.objf = d_objf; p.dz = d_dz; p.ldd = ldd;

@@ -30,3 +30,21 @@ def test_layer_norm():
         b = lambda x=P, ldx=C, dy=2 * P, lddy=C, sc=3 * P, m=4 * P, i=5 * P, dx=6 * P, lddx=C, ds=7 * P, do=8 * P: L.k3_layer_norm_backward(dtype, x, ldx, dy, lddy, sc, m, i, dx, lddx, ds, do, 0, 9 * P, n, R, C, None)  # noqa: E731
         for at in (P + size, 2 * P + size, P + size * (R * C - 1), 2 * P - size, 3 * P, 4 * P, 5 * P + 4 * R - size, 7 * P, 8 * P + 4 * C - size): refused(b(dx=at), "lies on")
         for k in (dict(dx=P, lddx=C + 1), dict(dx=2 * P, lddx=C + 8), dict(dx=P, ldx=C + 1), dict(dx=2 * P, lddy=C + 1), dict(ds=8 * P), dict(do=7 * P + 4 * C - 4)): refused(b(**k), "lies on")
+
+def test_label_scores():
+    L = _l.load(); R, C, N = 6, 40, 4
+    for dtype, size in ((0, 4), (1, 2), (2, 2)):
+        f = lambda y=2 * P, lp=3 * P, h=4 * P, st=5 * P, al=6 * P, ai=7 * P: L.k3_label_logprobs(dtype, P, C, y, lp, h, st, N, al, ai, None, 0, R, C, None)  # noqa: E731
+        for k, n in (("lp", R), ("h", R), ("st", 2 * R), ("al", N * R), ("ai", N * R)):
+            for at in (P, P + size * R * C - 4, P - 4 * n + 4, 2 * P, 2 * P + 4 * R - 4): refused(f(**{k: at}), "lies on")
+        g = lambda z=P, ld=C, dz=8 * P, ldd=C: L.k3_label_logprobs_deriv(dtype, z, ld, 2 * P, 3 * P, 4 * P, 5 * P, 6 * P, dz, ldd, R, C, None)  # noqa: E731
+        for at in (P + size, P - size, P + size * (R * C - 1), 2 * P, 3 * P + 8 * R - size, 4 * P, 5 * P, 6 * P + 4 * R - size): refused(g(dz=at), "lies on")
+        refused(g(dz=P, ldd=C + 1), "lies on"); refused(g(dz=P, ld=C + 8), "lies on"); refused(g(ld=100, ldd=100, dz=P + size * (C - 1)), "lies on")
+
+def test_distillation():
+    L = _l.load(); R, C, N = 6, 40, 4
+    for dtype, size in ((0, 4), (1, 2), (2, 2)):
+        f = lambda z=P, ld=C, v=2 * P, i=3 * P, w=4 * P, o=5 * P, dz=6 * P, ldd=C: L.k3_distill_objf_and_deriv(dtype, 1.0, z, ld, v, N, i, N, N, w, o, dz, ldd, None, 0, R, C, None)  # noqa: E731
+        for at in (P + size, P - size, P + size * (R * C - 1), 2 * P, 2 * P + size * (R * N - 1), 3 * P + 4 * R * N - size, 4 * P, 5 * P): refused(f(dz=at), "lies on")
+        for at in (P, P + size * R * C - 4, 2 * P, 3 * P + 4, 4 * P, 6 * P): refused(f(o=at), "lies on")
+        refused(f(dz=P, ldd=C + 1), "lies on"); refused(f(dz=P, ld=C + 8), "lies on"); refused(f(ld=100, ldd=100, dz=P + size * (C - 1)), "lies on")

@@ -40,3 +40,15 @@ def test_layer_norm_within_one_buffer():
             LayerNormPerRow(x, vectors[0], vectors[1], 1e-5, y, stats[0], stats[1]); DiffLayerNormPerRow(x, dy, vectors[0], stats[0], stats[1], dx, vectors[2], vectors[3])      # the vectors are neighbours too
             assert torch.equal(y, oy) and torch.equal(stats[0], om) and torch.equal(stats[1], oi) and torch.equal(dx, odx) and torch.equal(vectors[2], ods) and torch.equal(vectors[3], odo) and torch.equal(x, ox) and torch.equal(dy, ody)
             DiffLayerNormPerRow(x, dy, vectors[0], stats[0], stats[1], dy); assert torch.equal(dy, odx); LayerNormPerRow(x, vectors[0], vectors[1], 1e-5, x); assert torch.equal(x, oy)
+
+def test_scores_and_distillation_within_one_buffer():
+    from kaldi_amd.objective import LabelLogProbs, DiffLabelLogProbs, ComputeDistillObjfAndDeriv, DistillationOptions
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        for R, C, gap in ((50, 136, 0), (37, 19, 3), (1, 6024, 0), (9, 20011, 1), (2, 140001, 0)):
+            g = generator(C); z, dz, v, dd = beside((R, C), (R, C), (R, 5), (R, C), dtype=dtype, gap=gap); z.copy_(torch.randn(R, C, generator=g, device="cuda")); v.copy_(torch.randn(R, 5, generator=g, device="cuda"))
+            i = torch.randint(-1, C, (R, 5), generator=g, device="cuda").to(torch.int32); y = i[:, 0].contiguous(); vectors = torch.rand(6, R, generator=g, device="cuda"); st = torch.empty(R, 2, device="cuda")
+            oz, ov, o = z.clone(), v.clone(), [t.clone() for t in vectors]; odz, odd, ost = torch.empty_like(z.contiguous()), torch.empty_like(z.contiguous()), torch.empty_like(st); opt = DistillationOptions(2.0)
+            LabelLogProbs(oz, y, o[0], o[1], ost); DiffLabelLogProbs(oz, y, ost, o[1], o[2], o[3], odz); ComputeDistillObjfAndDeriv(opt, oz, ov, i, o[4], o[5], odd)
+            LabelLogProbs(z, y, vectors[0], vectors[1], st); DiffLabelLogProbs(z, y, st, vectors[1], vectors[2], vectors[3], dz); ComputeDistillObjfAndDeriv(opt, z, v, i, vectors[4], vectors[5], dd)
+            assert torch.equal(vectors, torch.stack(o)) and torch.equal(st, ost) and torch.equal(dz, odz) and torch.equal(dd, odd) and torch.equal(z, oz) and torch.equal(v, ov)
+            DiffLabelLogProbs(z, y, st, vectors[1], vectors[2], vectors[3], z); assert torch.equal(z, odz); z.copy_(oz); ComputeDistillObjfAndDeriv(opt, z, v, i, vectors[4], vectors[5], z); assert torch.equal(z, odd)
