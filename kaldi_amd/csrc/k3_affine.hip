@@ -542,7 +542,7 @@ Plan plan_product(int m, int n, int k) {
   for (int size = 0; size < 4; size++) {
     const Size &z = kSizes[size];
     const long long tm = (m + z.bm - 1) / z.bm, tn = (n + z.bn - 1) / z.bn, tiles = tm * tn, steps = std::max(1, (k + kStep - 1) / kStep);
-    if (tiles > 1 << 28) continue;
+    if ((tiles + 2 * z.slots) * (size == 3 ? 512 : 256) >= 1ll << 32) continue;      // (threads of a launch)
     const auto round = [&](long long units, double each) { return (each + 2.0) * std::max(z.alone, (double)((units + 255) / 256) * z.shared); };
     const auto rounds = [&](long long units, double each) { return (units / z.slots) * round(z.slots, each) + (units % z.slots ? round(units % z.slots, each) : 0.0); };
     const auto consider = [&](long long whole, long long units, double us) {
@@ -577,6 +577,7 @@ template <typename T, bool A_ACROSS, bool B_ACROSS, bool DIRECT> void launch_pro
 template <bool ACROSS> bool direct_ok(const void *p, long long ld, int rows) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld <= 1 << 22 && (!ACROSS || rows % 8 == 0); }
 template <typename T, bool A_ACROSS, bool B_ACROSS> int run_product(Product p, void *workspace, hipStream_t st) {
   const Plan pl = plan_product(p.m, p.n, p.k);
+  K3_REQUIRE(pl.whole + pl.units > 0, "k3_affine: matrix too large");
   p.tiles_m = pl.tiles_m; p.tiles_n = pl.tiles_n; p.whole = pl.whole; p.units = pl.units; p.steps = pl.steps;
   p.partial = (float *)workspace;
   if (direct_ok<A_ACROSS>(p.a, p.lda, p.m) && direct_ok<B_ACROSS>(p.b, p.ldb, p.n)) launch_product<T, A_ACROSS, B_ACROSS, true>(pl, p, st);

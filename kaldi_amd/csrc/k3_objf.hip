@@ -241,7 +241,7 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
   __shared__ float sh[4 * NW];
   __shared__ TopShared<NW> top_sh[RPB];
   const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x, sub = NW == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-  const long long item = (long long)blockIdx.x * RPB + sub;
+  const long long item = block_number() * RPB + sub;
   if (item >= (long long)p.rows * p.splits) return;      // (NW = 1: a whole wavefront, and no barrier spans wavefronts)
   const long long row = item / p.splits;
   const int part = (int)(item - row * p.splits), begin = part * p.span, end = min(p.cols, begin + p.span);
@@ -310,7 +310,8 @@ __device__ inline void join_parts(const Partial *part, int splits, float a, floa
 template <typename T> __global__ __launch_bounds__(256) void k3_row_scores_join_kernel(ScoreArgs p) {
   constexpr int E = kMaxSplits * kMaxTop / 256;
   __shared__ TopShared<4> top_sh;
-  const long long row = blockIdx.x;
+  const long long row = block_number();
+  if (row >= p.rows) return;
   int y;
   const bool has_label = label_of(p, row, y);
   const float label_value = has_label ? to_f32(((const T *)p.z)[row * p.ld + y]) : 0.0f;
@@ -343,7 +344,7 @@ template <typename T> __global__ __launch_bounds__(256) void k3_row_scores_join_
 template <typename T> __global__ __launch_bounds__(256) void k3_label_deriv_kernel(const T *z, long long ld, const int *labels, const float *stats, const float *entropy,
     const float *log_prob_deriv, const float *entropy_deriv, T *dz, long long ldd, int cols, int segments, long long items) {
   constexpr int N = Chunk<T>::N, E = 4;
-  const long long item = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long item = block_number() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= items) return;
   const long long row = item / segments;
   const int begin = (int)(item - row * segments) * (64 * E * N), end = min(cols, begin + 64 * E * N);
@@ -417,7 +418,7 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
   __shared__ float sh[6 * NW];
   extern __shared__ Entry entries[];
   const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x, sub = NW == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-  const long long row = (long long)blockIdx.x * RPB + sub;
+  const long long row = block_number() * RPB + sub;
   if (row >= p.rows) return;      // (NW = 1: a whole wavefront, and no barrier spans wavefronts)
   Entry *entry = entries + sub * p.top;
   const float teacher_max = read_teacher<T>(p, row, entry, t, 64 * NW);
@@ -467,7 +468,8 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
 // rows in parts: the objective, and what the derivative needs of a row: coef = {M, -w T / s, w T, whether it is not zero}, prob = its teacher's probabilities
 template <typename T> __global__ __launch_bounds__(64) void k3_distill_join_kernel(DistillArgs p) {
   extern __shared__ Entry entries[];
-  const long long row = blockIdx.x;
+  const long long row = block_number();
+  if (row >= p.rows) return;
   const int t = threadIdx.x;
   const float teacher_max = read_teacher<T>(p, row, entries, t, 64);
   const Teacher teacher = teacher_softmax<T, 1>(p, row, entries, teacher_max, t, nullptr);
@@ -483,8 +485,9 @@ template <typename T> __global__ __launch_bounds__(64) void k3_distill_join_kern
 }
 template <typename T> __global__ __launch_bounds__(256) void k3_distill_deriv_kernel(DistillArgs p, int segments) {
   constexpr int N = Chunk<T>::N, E = 4, SEG = 256 * E * N;
-  const long long row = blockIdx.x / segments;
-  const int begin = (int)(blockIdx.x - row * segments) * SEG, end = min(p.cols, begin + SEG), t = threadIdx.x;
+  const long long row = block_number() / segments;
+  if (row >= p.rows) return;
+  const int begin = (int)(block_number() - row * segments) * SEG, end = min(p.cols, begin + SEG), t = threadIdx.x;
   const T *z = (const T *)p.z + row * p.ld;
   T *dz = (T *)p.dz + row * p.ldd;
   const int *index = p.indexes + row * p.ld_indexes;
@@ -551,10 +554,10 @@ template <typename T> void split_rows(int rows, int cols, int &splits, int &span
 template <typename T> int launch_scores(ScoreArgs p, hipStream_t st) {
   const Shape s = shape_of<T>(std::min(p.cols, p.span), 1, 4);
   const long long items = (long long)p.rows * p.splits, blocks = s.nw == 1 ? (items + 3) / 4 : items;
-  K3_REQUIRE(s.e && blocks < (1ll << 31), "k3_objf: matrix too large");
+  K3_REQUIRE(s.e && blocks <= kMostGroups, "k3_objf: matrix too large");
   const auto launch = [&](auto nw, auto e) {
     constexpr int NW = decltype(nw)::value, E = decltype(e)::value;
-    hipLaunchKernelGGL((k3_row_scores_kernel<T, NW, E>), dim3((unsigned)blocks), dim3(NW == 1 ? 256 : 64 * NW), 0, st, p);
+    hipLaunchKernelGGL((k3_row_scores_kernel<T, NW, E>), grid_of(blocks, 256), dim3(NW == 1 ? 256 : 64 * NW), 0, st, p);
   };
   if (s.nw == 1) with_chunks<1>(s.e, launch);
   else with_chunks<4>(s.e, launch);
@@ -578,7 +581,7 @@ template <typename T> int label_logprobs(ScoreArgs p, void *workspace, hipStream
   p.part_col = (int *)w;
   const int rc = launch_scores<T>(p, st);
   if (rc) return rc;
-  hipLaunchKernelGGL((k3_row_scores_join_kernel<T>), dim3((unsigned)p.rows), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((k3_row_scores_join_kernel<T>), grid_of(p.rows, 256), dim3(256), 0, st, p);
   K3_HIP_CHECK(hipGetLastError());
   return K3_OK;
 }
@@ -596,7 +599,7 @@ template <typename T> int distill(DistillArgs p, void *workspace, hipStream_t st
   if (s.e) {
     const auto launch = [&](auto nw, auto e) {
       constexpr int NW = decltype(nw)::value, E = decltype(e)::value, RPB = NW == 1 ? 4 : 1;
-      hipLaunchKernelGGL((k3_distill_kernel<T, NW, E>), dim3((unsigned)((p.rows - 1) / RPB + 1)), dim3(NW == 1 ? 256 : 64 * NW), sizeof(Entry) * RPB * p.top, st, p);
+      hipLaunchKernelGGL((k3_distill_kernel<T, NW, E>), grid_of((p.rows - 1) / RPB + 1, NW == 1 ? 256 : 64 * NW), dim3(NW == 1 ? 256 : 64 * NW), sizeof(Entry) * RPB * p.top, st, p);
     };
     if (s.nw == 1) with_chunks<1>(s.e, launch);
     else if (s.nw == 4) with_chunks<4>(s.e, launch);
@@ -616,13 +619,13 @@ template <typename T> int distill(DistillArgs p, void *workspace, hipStream_t st
   p.coef = (float4 *)w;
   p.prob = (float *)(w + (int64_t)p.rows * 16);
   const int segments = (p.cols + 256 * 4 * Chunk<T>::N - 1) / (256 * 4 * Chunk<T>::N);
-  K3_REQUIRE((long long)p.rows * segments < (1ll << 31), "k3_distill_objf_and_deriv: matrix too large");
+  K3_REQUIRE((long long)p.rows * segments <= kMostGroups, "k3_distill_objf_and_deriv: matrix too large");
   const int rc = launch_scores<T>(sc, st);
   if (rc) return rc;
-  hipLaunchKernelGGL((k3_distill_join_kernel<T>), dim3((unsigned)p.rows), dim3(64), sizeof(Entry) * p.top, st, p);
+  hipLaunchKernelGGL((k3_distill_join_kernel<T>), grid_of(p.rows, 64), dim3(64), sizeof(Entry) * p.top, st, p);
   K3_HIP_CHECK(hipGetLastError());
   if (p.dz) {
-    hipLaunchKernelGGL((k3_distill_deriv_kernel<T>), dim3((unsigned)(p.rows * segments)), dim3(256), 0, st, p, segments);
+    hipLaunchKernelGGL((k3_distill_deriv_kernel<T>), grid_of((long long)p.rows * segments, 256), dim3(256), 0, st, p, segments);
     K3_HIP_CHECK(hipGetLastError());
   }
   return K3_OK;
@@ -673,8 +676,8 @@ extern "C" int k3_label_logprobs_deriv(int32_t dtype, const void *d_z, int64_t l
 #define K3_LABEL_DERIV(T)                                                                                                                            \
   const int segments = (cols + 256 * Chunk<T>::N - 1) / (256 * Chunk<T>::N);                                                                         \
   const long long items = (long long)rows * segments, blocks = (items + 3) / 4;                                                                      \
-  K3_REQUIRE(blocks < (1ll << 31), "k3_label_logprobs_deriv: matrix too large");                                                                     \
-  hipLaunchKernelGGL((k3_label_deriv_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const T *)d_z, (long long)ld, d_labels, \
+  K3_REQUIRE(blocks <= kMostGroups, "k3_label_logprobs_deriv: matrix too large");                                                                    \
+  hipLaunchKernelGGL((k3_label_deriv_kernel<T>), grid_of(blocks, 256), dim3(256), 0, (hipStream_t)stream, (const T *)d_z, (long long)ld, d_labels,   \
                     d_stats, d_entropy, d_log_prob_deriv, d_entropy_deriv, (T *)d_dz, (long long)ldd, cols, segments, items)
   K3_FOR_DTYPE(dtype, K3_LABEL_DERIV);
   K3_HIP_CHECK(hipGetLastError());

@@ -133,6 +133,14 @@ template <int NW> __device__ inline void block_sum2(float &a, float &b, float *s
   }
 }
 
+// A launch has less than 2^32 threads along one dimension: more workgroups go in several rows of 2^20 (those behind the last one return)
+constexpr long long kMostGroups = (1ll << 20) * 65535;
+inline dim3 grid_of(long long blocks, int threads) {
+  if (blocks * threads < (1ll << 32)) return dim3((unsigned)blocks);
+  return dim3(1u << 20, (unsigned)((blocks + (1 << 20) - 1) >> 20));
+}
+__device__ inline long long block_number() { return blockIdx.x + (long long)blockIdx.y * gridDim.x; }
+
 inline bool dtype_ok(int dtype) { return dtype >= K3_F32 && dtype <= K3_BF16; }
 inline size_t dtype_size(int dtype) { return dtype == K3_F32 ? 4 : 2; }
 
