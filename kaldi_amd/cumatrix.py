@@ -40,7 +40,7 @@ def _vec(t, n, i, name, dtype=_F32):
     _refuse(f"{name}: a contiguous {dtype} tensor of {n} elements on device {i} is wanted")
 def _table(t, r, c, i, name, dtype=_F32):
     """pointer of a contiguous [r, c] tensor on device i (None: null)"""
-    if t is not None and t.shape != (r, c): _refuse(f"{name}: a tensor of shape {(r, c)} is wanted, not {tuple(t.shape)}")
+    if t is not None and getattr(t, "shape", None) != (r, c): _refuse(f"{name}: a tensor of shape {(r, c)} is wanted, not {tuple(getattr(t, 'shape', ()))}")
     return _vec(t, r * c, i, name, dtype)
 def _workspace(n, i):
     """n bytes on device i, of the current stream (or of the graph that is being captured); None for none"""

@@ -10,7 +10,8 @@ def LabelLogProbs(nnet_output, labels, log_prob=None, entropy=None, stats=None, 
     row's n most probable columns, best first, equal ones by column.  -inf in nnet_output = a column that cannot be; a row with a NaN or +inf has NaN scores and alternatives -1."""
     dt, z, ld, r, c, i = _rows(nnet_output, "nnet_output")
     alt = alt_log_probs if alt_log_probs is not None else alt_labels
-    n = 0 if alt is None else alt.shape[-1]
+    try: n = 0 if alt is None else alt.shape[-1]
+    except (AttributeError, IndexError): _refuse("alternatives: tensors of shape [rows, n] are wanted")
     if n > 64: _refuse(f"alternatives: {n}, at most 64 are kept")
     L = _l.load(); nw = L.k3_label_logprobs_workspace(dt, r, c, n); w = _workspace(nw, i)
     _run(i, L.k3_label_logprobs, dt, z, ld, _vec(labels, r, i, "labels", _I32), _vec(log_prob, r, i, "log_prob"), _vec(entropy, r, i, "entropy"), _table(stats, r, 2, i, "stats"), n,
@@ -37,7 +38,7 @@ def ComputeDistillObjfAndDeriv(opts, nnet_output, teacher_values, teacher_indexe
     vt, v, ldv, vr, n, vi = _rows(teacher_values, "teacher_values")
     if vr != r or vt != dt or vi != i: _refuse(f"teacher_values: {vr} rows of type {vt} on device {vi} do not go with {r} of type {dt} on device {i}")
     t = teacher_indexes
-    if t.dtype is not _I32 or t.shape != (r, n) or t.get_device() != i: _refuse(f"teacher_indexes: an int32 matrix of shape {(r, n)} on device {i} is wanted")
+    if getattr(t, "dtype", None) is not _I32 or t.shape != (r, n) or t.get_device() != i: _refuse(f"teacher_indexes: an int32 matrix of shape {(r, n)} on device {i} is wanted")
     s0, s1 = t.stride()
     if r <= 1: s0 = n
     if (s1 != 1 and n > 1) or s0 < n: _refuse(f"teacher_indexes: rows must be contiguous and must not overlap (strides {s0}, {s1})")
