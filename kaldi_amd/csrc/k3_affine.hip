@@ -76,14 +76,8 @@ struct Epilogue {
   int act;
 };
 // C [m x n] over k contraction steps, in tiles of `steps` LDS tiles of 64 of them.  The first `whole` tiles are one workgroup's each.  Those behind them (what would leave most of the chip
-// idle) are, one behind the other, cut into `units` runs of equal length, one workgroup's each: a tile that lies in one run is finished by it, of the others the float32 sums of every
-// run's piece go to partial [run + tile][BM][BN] (a number of its own for every piece) and are joined by k3_affine_join_kernel.
-struct Product {
-  const void *a; long long lda; const void *b; long long ldb; int m, n, k; int tiles_m, tiles_n, whole, units, steps; float *partial; Epilogue e;
-  __device__ inline int rest() const { return tiles_m * tiles_n - whole; }
-  __device__ inline long long run_start(int u) const { return (long long)u * ((long long)rest() * steps) / units; }
-  __device__ inline int run_of(long long at) const { return (int)(((at + 1) * units - 1) / ((long long)rest() * steps)); }      // which run a step lies in
-};
+// idle) are cut into `parts` pieces of their steps each, one workgroup's each: their float32 sums go to partial [tile * parts + part][BM][BN] and are joined by k3_affine_join_kernel.
+struct Product { const void *a; long long lda; const void *b; long long ldb; int m, n, k; int tiles_m, tiles_n, whole, parts, steps; float *partial; Epilogue e; };
 
 typedef float f8 __attribute__((ext_vector_type(8)));
 
@@ -241,9 +235,12 @@ __device__ inline void place(const Product &p, int tile, int &tm, int &tn) {
   tn = panel * 8 + rest - tm * width;
 }
 
-// BM x BN outputs per workgroup of WM x WN wavefronts, over LDS tiles of 64 contraction steps, two of them: one is loaded while the other is multiplied.  PIPED (the size of which a compute
+// BM x BN outputs per workgroup of WM x WN wavefronts, over STAGES LDS tiles of 64 contraction steps: one is multiplied while the others are loaded.  PIPED (the size of which a compute
 // unit holds one workgroup): a tile is two halves of 32 steps for the matrix instructions, and the fragments of a half are read from LDS among the instructions of the half before it, those
-// of the next tile's first half too: the one barrier per tile stands between the halves, where every wavefront has read all of this tile (which the loads issued behind the barrier then overwrite) and the next one has arrived.
+// of the next tile's first half too: the one barrier per tile stands between the halves, where every wavefront has read all of this tile (which the loads issued behind the barrier then
+// overwrite) and the next one has arrived.
+// Where an operand is ACROSS, the compiler takes its transposing LDS reads to depend on every load into LDS under way and waits for all of them first: the loads of a tile, issued right
+// before those reads, then have no time but what the compute unit's other wavefronts take, and the rings of 3 and 4 tiles hold nothing in flight.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_ACROSS, bool B_ACROSS, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product p) {
   constexpr int THREADS = 64 * WM * WN, MI = BM / WM / 16, NI = BN / WN / 16, BK = 64;
@@ -255,198 +252,183 @@ __global__ __launch_bounds__(64 * WM * WN) void k3_affine_product_kernel(Product
   using LB = Loader<T, BN, BK, B_ACROSS, THREADS>;
   constexpr int kStage = TA::kBytes + TB::kBytes;
   __shared__ __attribute__((aligned(1024))) char lds[STAGES * kStage];
-  // workgroups go round the 8 XCDs: each XCD takes neighbouring tiles, which share operands in its L2; so do the runs of the last tiles
+  // workgroups go round the 8 XCDs: each XCD takes neighbouring tiles, which share operands in its L2; so do the parts of the last tiles
   const bool split = (int)blockIdx.x >= p.whole;
-  const int count = split ? p.units : p.whole, u = split ? blockIdx.x - p.whole : blockIdx.x;
+  const int count = split ? (int)gridDim.x - p.whole : p.whole, u = split ? blockIdx.x - p.whole : blockIdx.x;
   const int per = count / 8, extra = count % 8, x = u % 8, unit = x * per + min(x, extra) + u / 8;
-  const long long run_end = split ? p.run_start(unit + 1) : 0;
-  long long at = split ? p.run_start(unit) : 0;
-  do {      // one round per piece of a tile: this workgroup's tile, or what its run has of one
-    const int t = split ? (int)(at / p.steps) : 0, step0 = split ? (int)(at - (long long)t * p.steps) : 0, step1 = split ? (int)min((long long)p.steps, step0 + run_end - at) : p.steps;
-    const bool piece = step0 > 0 || step1 < p.steps;
-    at += step1 - step0;
-    int thread = threadIdx.x;
-    asm volatile("" : "+v"(thread));      // (what is made of it is made anew for every piece, and takes no registers from the loop below)
-    const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), wm = wave / WN, wn = wave % WN;
-    int tm, tn;
-    place(p, split ? p.whole + t : unit, tm, tn);
-    const int first = step0 * BK, end = min(p.k, step1 * BK);
-    const int direct = DIRECT ? (end - first) / BK : 0, steps = (end - first + BK - 1) / BK;
-    LA la{(const T *)p.a, p.lda, tm * BM, p.m, p.k, wave, lane};
-    LB lb{(const T *)p.b, p.ldb, tn * BN, p.n, p.k, wave, lane};
-    f4 acc[MI][NI] = {};
-    typedef typename Half<T>::frag frag;
-    const auto read = [&](const char *ta, int ks, frag (&a)[MI], frag (&b)[NI]) {
+  const int t = split ? unit / p.parts : unit, part = split ? unit - t * p.parts : 0;
+  const int step0 = split ? (int)((long long)part * p.steps / p.parts) : 0, step1 = split ? (int)((long long)(part + 1) * p.steps / p.parts) : p.steps;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  int tm, tn;
+  place(p, split ? p.whole + t : t, tm, tn);
+  const int first = step0 * BK, end = min(p.k, step1 * BK);
+  const int direct = DIRECT ? (end - first) / BK : 0, steps = (end - first + BK - 1) / BK;
+  LA la{(const T *)p.a, p.lda, tm * BM, p.m, p.k, wave, lane};
+  LB lb{(const T *)p.b, p.ldb, tn * BN, p.n, p.k, wave, lane};
+  f4 acc[MI][NI] = {};
+  typedef typename Half<T>::frag frag;
+  const auto read = [&](const char *ta, int ks, frag (&a)[MI], frag (&b)[NI]) {
 #pragma unroll
-      for (int j = 0; j < NI; j++) b[j] = TB::template fragment<T>(ta + TA::kBytes, wn * (BN / WN) + j * 16, ks, lane);
+    for (int j = 0; j < NI; j++) b[j] = TB::template fragment<T>(ta + TA::kBytes, wn * (BN / WN) + j * 16, ks, lane);
 #pragma unroll
-      for (int i = 0; i < MI; i++) a[i] = TA::template fragment<T>(ta, wm * (BM / WM) + i * 16, ks, lane);
-    };
-    const auto multiply = [&](const frag (&a)[MI], const frag (&b)[NI]) {
+    for (int i = 0; i < MI; i++) a[i] = TA::template fragment<T>(ta, wm * (BM / WM) + i * 16, ks, lane);
+  };
+  const auto multiply = [&](const frag (&a)[MI], const frag (&b)[NI]) {
 #pragma unroll
-      for (int i = 0; i < MI; i++)
+    for (int i = 0; i < MI; i++)
 #pragma unroll
-        for (int j = 0; j < NI; j++) Half<T>::mfma(b[j], a[i], acc[i][j]);      // (n, m): a lane ends with 4 consecutive n of one m
-    };
-    // the order of a half: its loads and LDS reads spread over the first part of its matrix instructions
-    constexpr int READS = (A_ACROSS ? 2 : 1) * MI + (B_ACROSS ? 2 : 1) * NI;
-    const auto interleave = [&](auto loads) {
-      constexpr int L = decltype(loads)::value, PER = MI * NI / (READS + L) > 0 ? MI * NI / (READS + L) : 1;
+      for (int j = 0; j < NI; j++) Half<T>::mfma(b[j], a[i], acc[i][j]);      // (n, m): a lane ends with 4 consecutive n of one m
+  };
+  // the order of a half: its LDS reads spread over the first part of its matrix instructions
+  constexpr int READS = (A_ACROSS ? 2 : 1) * MI + (B_ACROSS ? 2 : 1) * NI, PER = MI * NI / READS > 0 ? MI * NI / READS : 1;
+  const auto interleave = [&]() {
 #pragma unroll
-      for (int i = 0; i < READS; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < L; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, MI * NI, 0);
-    };
-    if constexpr (DIRECT) {
-      if (direct) {
-        const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char *)lds;
-        la.start(first);
-        lb.start(first);
-        unsigned load = 0;      // where the next tile goes
-        const auto issue = [&](int) {
-          la.direct(lds0 + load);
-          lb.direct(lds0 + load + TA::kBytes);
-          load = load == (STAGES - 1) * kStage ? 0 : load + kStage;
+    for (int i = 0; i < READS; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, MI * NI, 0);
+  };
+  if constexpr (DIRECT) {
+    if (direct) {
+      const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char *)lds;
+      la.start(first);
+      lb.start(first);
+      unsigned load = 0;      // where the next tile goes
+      const auto issue = [&](int) {
+        la.direct(lds0 + load);
+        lb.direct(lds0 + load + TA::kBytes);
+        load = load == (STAGES - 1) * kStage ? 0 : load + kStage;
+      };
+      issue(0);
+      if constexpr (PIPED) {
+        frag a0[MI], b0[NI], a1[MI], b1[NI];
+        arrive<0>();
+        if (direct > 1) issue(1);
+        read(lds, 0, a0, b0);
+        const auto step = [&](int s, auto loads) {
+          read(lds + (s & 1) * kStage, 1, a1, b1);
+          multiply(a0, b0);
+          interleave();
+          arrive<0>();
+          if constexpr (decltype(loads)::value) issue(s);
+          __builtin_amdgcn_sched_barrier(0);      // (the loads at once: left to itself the compiler puts them behind most of the matrix instructions)
+          read(lds + ((s & 1) ^ 1) * kStage, 0, a0, b0);      // (behind the last tile: something from LDS, for nothing)
+          multiply(a1, b1);
+          interleave();
         };
-        issue(0);
-        if constexpr (PIPED) {
-          frag a0[MI], b0[NI], a1[MI], b1[NI];
-          __syncthreads();
-          if (direct > 1) issue(1);
-          read(lds, 0, a0, b0);
-          const auto step = [&](int s, auto loads) {
-            read(lds + (s & 1) * kStage, 1, a1, b1);
-            multiply(a0, b0);
-            interleave(std::integral_constant<int, 0>());
-            arrive<0>();
-            if constexpr (decltype(loads)::value) issue(s);
-            read(lds + ((s & 1) ^ 1) * kStage, 0, a0, b0);      // (behind the last tile: something from LDS, for nothing)
-            multiply(a1, b1);
-            interleave(loads);
-          };
-          int s = 0;
-          for (; s + 2 < direct; s++) step(s, std::integral_constant<int, LA::N + LB::N>());
-          for (; s < direct; s++) step(s, std::integral_constant<int, 0>());
-        } else {
-          // STAGES - 1 tiles are on their way while one is multiplied
+        int s = 0;
+        for (; s + 2 < direct; s++) step(s, std::true_type());
+        for (; s < direct; s++) step(s, std::false_type());
+      } else {
+        // STAGES - 1 tiles are on their way while one is multiplied
 #pragma unroll
-          for (int i = 1; i < STAGES - 1; i++) if (i < direct) issue(i);
-          unsigned now = 0;
-          for (int s = 0; s < direct; s++) {
-            if (s + STAGES - 2 < direct) arrive<(STAGES - 2) * (LA::N + LB::N)>();
-            else arrive<0>();
-            if (s + STAGES - 1 < direct) issue(s + STAGES - 1);
-            frag a[MI], b[NI];
+        for (int i = 1; i < STAGES - 1; i++) if (i < direct) issue(i);
+        unsigned now = 0;
+        for (int s = 0; s < direct; s++) {
+          if (s + STAGES - 2 < direct) arrive<(STAGES - 2) * (LA::N + LB::N)>();
+          else arrive<0>();
+          if (s + STAGES - 1 < direct) issue(s + STAGES - 1);
+          frag a[MI], b[NI];
 #pragma unroll
-            for (int ks = 0; ks < 2; ks++) {
-              read(lds + now, ks, a, b);
-              multiply(a, b);
-            }
-            now = now == (STAGES - 1) * kStage ? 0 : now + kStage;
+          for (int ks = 0; ks < 2; ks++) {
+            read(lds + now, ks, a, b);
+            multiply(a, b);
+          }
+          now = now == (STAGES - 1) * kStage ? 0 : now + kStage;
+        }
+      }
+      __syncthreads();
+    }
+  }
+  // what is left of the contraction (everything, where the operands' alignment does not allow the direct way): through registers, R tiles of them on their way
+  if (direct < steps) {
+    constexpr int R = DIRECT || BM >= 128 ? 1 : 3;      // (two of 128 x 128 would leave a compute unit one workgroup instead of two)
+    typename LA::chunk va[R][LA::N];
+    typename LB::chunk vb[R][LB::N];
+    la.fetch(first + direct * BK, va[0]);
+    lb.fetch(first + direct * BK, vb[0]);
+    la.store(lds, va[0]);
+    lb.store(lds + TA::kBytes, vb[0]);
+#pragma unroll
+    for (int r = 0; r < R; r++)
+      if (direct + 1 + r < steps) {
+        la.fetch(first + (direct + 1 + r) * BK, va[r]);
+        lb.fetch(first + (direct + 1 + r) * BK, vb[r]);
+      }
+    __syncthreads();
+    for (int s0 = direct; s0 < steps; s0 += R)
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const int s = s0 + r, now = (s - direct) & 1;
+        if (s >= steps) break;
+        frag a[MI], b[NI];
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+          read(lds + now * kStage, ks, a, b);
+          multiply(a, b);
+        }
+        if (s + 1 < steps) {
+          la.store(lds + (now ^ 1) * kStage, va[r]);
+          lb.store(lds + (now ^ 1) * kStage + TA::kBytes, vb[r]);
+          if (s + 1 + R < steps) {
+            la.fetch(first + (s + 1 + R) * BK, va[r]);
+            lb.fetch(first + (s + 1 + R) * BK, vb[r]);
           }
         }
         __syncthreads();
       }
-    }
-    // what is left of the contraction (everything, where the operands' alignment does not allow the direct way): through registers, R tiles of them on their way
-    if (direct < steps) {
-      constexpr int R = DIRECT || BM >= 128 ? 1 : 3;      // (two of 128 x 128 would leave a compute unit one workgroup instead of two)
-      typename LA::chunk va[R][LA::N];
-      typename LB::chunk vb[R][LB::N];
-      la.fetch(first + direct * BK, va[0]);
-      lb.fetch(first + direct * BK, vb[0]);
-      la.store(lds, va[0]);
-      lb.store(lds + TA::kBytes, vb[0]);
+  }
+  // The epilogue goes through LDS, a part of each wavefront's rows at a time (as many as its share of the tiles' memory holds): out of the accumulators' layout (4 columns of one of 16 rows
+  // per lane) into runs of whole rows, so that what is read and written beside it are lines.  A row's chunk c of 4 lies at c ^ a function of the row that differs among the 16 rows that are
+  // written at once.
+  constexpr int CW = BN / WN, Q = CW / 4, SHARE = (int)sizeof(lds) / (WM * WN) / 16 * 16, HOLD = SHARE / (CW * 4) / 16 * 16;
+  constexpr int PASS = HOLD >= BM / WM ? BM / WM : BM / WM / 2, STRIDE = 64 / (Q / 2), U = PASS / STRIDE;      // rows per pass, rows between a lane's, and rows per lane
+  static_assert(PASS >= 16 && PASS <= HOLD && (BM / WM) % PASS == 0 && U >= 1, "rows per pass");
+  f4 *mine = (f4 *)(lds + wave * SHARE);
+  const int m0 = tm * BM + wm * (BM / WM), n0 = tn * BN + wn * CW;
+  float *sums = p.partial + (long long)unit * (BM * BN) + wm * (BM / WM) * BN + wn * CW;
 #pragma unroll
-      for (int r = 0; r < R; r++)
-        if (direct + 1 + r < steps) {
-          la.fetch(first + (direct + 1 + r) * BK, va[r]);
-          lb.fetch(first + (direct + 1 + r) * BK, vb[r]);
-        }
-      __syncthreads();
-      for (int s0 = direct; s0 < steps; s0 += R)
+  for (int i0 = 0; i0 < MI; i0 += PASS / 16) {
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-          const int s = s0 + r, now = (s - direct) & 1;
-          if (s >= steps) break;
-          frag a[MI], b[NI];
+    for (int i = 0; i < PASS / 16; i++)
 #pragma unroll
-          for (int ks = 0; ks < 2; ks++) {
-            read(lds + now * kStage, ks, a, b);
-            multiply(a, b);
-          }
-          if (s + 1 < steps) {
-            la.store(lds + (now ^ 1) * kStage, va[r]);
-            lb.store(lds + (now ^ 1) * kStage + TA::kBytes, vb[r]);
-            if (s + 1 + R < steps) {
-              la.fetch(first + (s + 1 + R) * BK, va[r]);
-              lb.fetch(first + (s + 1 + R) * BK, vb[r]);
-            }
-          }
-          __syncthreads();
-        }
-    }
-    // The epilogue goes through LDS, a part of each wavefront's rows at a time (as many as its share of the tiles' memory holds): out of the accumulators' layout (4 columns of one of 16 rows
-    // per lane) into runs of whole rows, so that what is read and written beside it are lines.  A row's chunk c of 4 lies at c ^ a function of the row that differs among the 16 rows that are
-    // written at once.
-    constexpr int CW = BN / WN, Q = CW / 4, SHARE = (int)sizeof(lds) / (WM * WN) / 16 * 16, HOLD = SHARE / (CW * 4) / 16 * 16;
-    constexpr int PASS = HOLD >= BM / WM ? BM / WM : BM / WM / 2, STRIDE = 64 / (Q / 2), U = PASS / STRIDE;      // rows per pass, rows between a lane's, and rows per lane
-    static_assert(PASS >= 16 && PASS <= HOLD && (BM / WM) % PASS == 0 && U >= 1, "rows per pass");
-    f4 *mine = (f4 *)(lds + wave * SHARE);
-    const int m0 = tm * BM + wm * (BM / WM), n0 = tn * BN + wn * CW;
-    float *sums = p.partial + (long long)(unit + t) * (BM * BN) + wm * (BM / WM) * BN + wn * CW;
-#pragma unroll
-    for (int i0 = 0; i0 < MI; i0 += PASS / 16) {
-#pragma unroll
-      for (int i = 0; i < PASS / 16; i++)
-#pragma unroll
-        for (int j = 0; j < NI; j++) {
-          const int r = i * 16 + (lane & 15), c = j * 4 + (lane >> 4);
-          mine[r * Q + (c ^ (r / (16 / Q) & (Q - 1)))] = acc[i0 + i][j];
-        }
-      wave_fence();
-      const int r0 = lane / (Q / 2), c = lane % (Q / 2) * 2;      // this lane's first row and columns of the pass
-      const auto value = [&](int u) {
-        const int r = r0 + u * STRIDE, f = r / (16 / Q) & (Q - 1);
-        return __builtin_shufflevector(mine[r * Q + (c ^ f)], mine[r * Q + ((c + 1) ^ f)], 0, 1, 2, 3, 4, 5, 6, 7);
-      };
-      if (piece) {
+      for (int j = 0; j < NI; j++) {
+        const int r = i * 16 + (lane & 15), c = j * 4 + (lane >> 4);
+        mine[r * Q + (c ^ (r / (16 / Q) & (Q - 1)))] = acc[i0 + i][j];
+      }
+    wave_fence();
+    const int r0 = lane / (Q / 2), c = lane % (Q / 2) * 2;      // this lane's first row and columns of the pass
+    const auto value = [&](int u) {
+      const int r = r0 + u * STRIDE, f = r / (16 / Q) & (Q - 1);
+      return __builtin_shufflevector(mine[r * Q + (c ^ f)], mine[r * Q + ((c + 1) ^ f)], 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    if (split) {
 #pragma unroll 1
-        for (int u = 0; u < U; u++) *(f8 *)(sums + (i0 * 16 + r0 + u * STRIDE) * BN + c * 4) = value(u);
-      } else if (n0 + CW <= p.n && p.e.act <= kRelu) finish_rows<T, U>(p.e, m0 + i0 * 16 + r0, STRIDE, p.m, n0 + c * 4, value);
-      else
+      for (int u = 0; u < U; u++) *(f8 *)(sums + (i0 * 16 + r0 + u * STRIDE) * BN + c * 4) = value(u);
+    } else if (n0 + CW <= p.n && p.e.act <= kRelu) finish_rows<T, U>(p.e, m0 + i0 * 16 + r0, STRIDE, p.m, n0 + c * 4, value);
+    else
 #pragma unroll 1
-        for (int u = 0; u < U; u++) {
-          const long long row = m0 + i0 * 16 + r0 + u * STRIDE;
-          if (row < p.m && n0 + c * 4 < p.n) finish<T>(p.e, row, n0 + c * 4, p.n - n0 - c * 4, value(u));
-        }
-      wave_fence();
-    }
-    if (split) __syncthreads();      // (LDS is the next piece's)
-  } while (at < run_end);
+      for (int u = 0; u < U; u++) {
+        const long long row = m0 + i0 * 16 + r0 + u * STRIDE;
+        if (row < p.m && n0 + c * 4 < p.n) finish<T>(p.e, row, n0 + c * 4, p.n - n0 - c * 4, value(u));
+      }
+    wave_fence();
+  }
 }
 
 // the sums of a cut tile's pieces, in their order, and the epilogue: 8 columns per thread
 template <typename T> __global__ __launch_bounds__(256) void k3_affine_join_kernel(Product p, int bm, int bn) {
   const int groups = bm * bn / 2048, t = blockIdx.x / groups, e = (blockIdx.x - t * groups) * 256 + threadIdx.x, r = e / (bn / 8), c = e % (bn / 8) * 8;
-  const int first = p.run_of((long long)t * p.steps), last = p.run_of((long long)(t + 1) * p.steps - 1);
-  if (first == last) return;      // in one run, which has finished it
   int tm, tn;
   place(p, p.whole + t, tm, tn);
   const long long row = (long long)tm * bm + r;
   const int col = tn * bn + c;
   if (row >= p.m || col >= p.n) return;
-  const float *in = p.partial + (long long)(first + t) * bm * bn + r * bn + c;
+  const float *in = p.partial + (long long)t * p.parts * bm * bn + r * bn + c;
   f8 v = *(const f8 *)in;
 #pragma unroll 4
-  for (int u = 1; u <= last - first; u++) v += *(const f8 *)(in + (long long)u * bm * bn);
+  for (int u = 1; u < p.parts; u++) v += *(const f8 *)(in + (long long)u * bm * bn);
   finish<T>(p.e, row, col, p.n - col, v);
 }
 
@@ -531,11 +513,11 @@ __global__ __launch_bounds__(1024) void k3_affine_bias_join_kernel(const float *
 struct Size { int bm, bn, slots; double alone, shared; };
 const Size kSizes[4] = {{32, 64, 1536, 0.25, 0.115}, {64, 64, 1024, 0.3, 0.19}, {128, 128, 512, 0.7, 0.5}, {256, 256, 256, 1.5, 1.7}};
 constexpr int kStep = 64;
-struct Plan { int size, tiles_m, tiles_n, whole, units, steps; int64_t bytes; };
+struct Plan { int size, tiles_m, tiles_n, whole, parts, steps; int64_t bytes; };      // parts 0: no tile is cut
 
-// The size and the runs of the last tiles that cost least by a model of rounds over the chip: rounds of whole tiles, the runs, and their pieces' way through memory.  The runs are a whole
-// number per tile: 256 equal runs over 72 tiles of 400 steps keep every unit busy, but no two of them are then at the same step and share an operand, and a weight derivative of
-// 6024 x 768 over 25600 rows took 346 us against 293 in 3 runs per tile.
+// The size, and the parts of the last tiles, that cost least by a model of rounds over the chip: rounds of whole tiles, the parts, and their sums' way through memory.  A whole number of
+// parts per tile: 256 equal runs over 72 tiles of 400 steps keep every unit busy, but no two of them are then at the same step and share an operand, and a weight derivative of
+// 6024 x 768 over 25600 rows took 346 us against 293 in 3 parts per tile.
 Plan plan_product(int m, int n, int k) {
   Plan best{};
   double least = 1e300;
@@ -545,27 +527,25 @@ Plan plan_product(int m, int n, int k) {
     if ((tiles + 2 * z.slots) * (size == 3 ? 512 : 256) >= 1ll << 32) continue;      // (threads of a launch)
     const auto round = [&](long long units, double each) { return (each + 2.0) * std::max(z.alone, (double)((units + 255) / 256) * z.shared); };
     const auto rounds = [&](long long units, double each) { return (units / z.slots) * round(z.slots, each) + (units % z.slots ? round(units % z.slots, each) : 0.0); };
-    const auto consider = [&](long long whole, long long units, double us) {
-      if (us < least) {
-        least = us;
-        const long long pieces = units ? units + tiles - whole : 0;
-        best = {size, (int)tm, (int)tn, (int)whole, (int)units, (int)steps, (int64_t)pieces * z.bm * z.bn * 4};
-      }
+    const auto consider = [&](long long whole, int parts, double us) {
+      if (us >= least) return;
+      least = us;
+      best = {size, (int)tm, (int)tn, (int)whole, parts, (int)steps, (int64_t)(tiles - whole) * parts * z.bm * z.bn * 4};
     };
     consider(tiles, 0, rounds(tiles, steps));
     const long long whole = tiles / z.slots * z.slots, rest = tiles - whole;
     if (rest == 0) continue;
-    for (int parts = 2; parts <= 16 && rest * parts <= 2 * z.slots && steps >= 2 * parts; parts++) {      // (a whole number of runs per tile)
+    for (int parts = 2; parts <= 16 && rest * parts <= 2 * z.slots && steps >= 2 * parts; parts++) {
       const long long units = rest * parts;
       const double bytes = (double)units * z.bm * z.bn * 4, each = (double)steps / parts;
-      consider(whole, units, rounds(whole, steps) + rounds(units, each) + 3.0 + 2.0 * bytes / 5e6);
+      consider(whole, parts, rounds(whole, steps) + rounds(units, each) + 3.0 + 2.0 * bytes / 5e6);
     }
   }
   return best;
 }
 
 template <typename T, bool A_ACROSS, bool B_ACROSS, bool DIRECT> void launch_product(const Plan &pl, const Product &p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.whole + p.units));
+  const dim3 grid((unsigned)(p.whole + (p.tiles_m * p.tiles_n - p.whole) * p.parts));
   switch (pl.size) {
     case 0: hipLaunchKernelGGL((k3_affine_product_kernel<T, 32, 64, 1, 4, 4, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
     case 1: hipLaunchKernelGGL((k3_affine_product_kernel<T, 64, 64, 2, 2, 3, A_ACROSS, B_ACROSS, DIRECT>), grid, dim3(256), 0, st, p); return;
@@ -577,8 +557,8 @@ template <typename T, bool A_ACROSS, bool B_ACROSS, bool DIRECT> void launch_pro
 template <bool ACROSS> bool direct_ok(const void *p, long long ld, int rows) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld <= 1 << 22 && (!ACROSS || rows % 8 == 0); }
 template <typename T, bool A_ACROSS, bool B_ACROSS> int run_product(Product p, void *workspace, hipStream_t st) {
   const Plan pl = plan_product(p.m, p.n, p.k);
-  K3_REQUIRE(pl.whole + pl.units > 0, "k3_affine: matrix too large");
-  p.tiles_m = pl.tiles_m; p.tiles_n = pl.tiles_n; p.whole = pl.whole; p.units = pl.units; p.steps = pl.steps;
+  K3_REQUIRE(pl.steps > 0, "k3_affine: matrix too large");
+  p.tiles_m = pl.tiles_m; p.tiles_n = pl.tiles_n; p.whole = pl.whole; p.parts = pl.parts; p.steps = pl.steps;
   p.partial = (float *)workspace;
   if (direct_ok<A_ACROSS>(p.a, p.lda, p.m) && direct_ok<B_ACROSS>(p.b, p.ldb, p.n)) launch_product<T, A_ACROSS, B_ACROSS, true>(pl, p, st);
   else launch_product<T, A_ACROSS, B_ACROSS, false>(pl, p, st);
