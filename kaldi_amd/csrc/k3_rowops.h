@@ -139,7 +139,7 @@ inline dim3 grid_of(long long blocks, int threads) {
   if (blocks * threads < (1ll << 32)) return dim3((unsigned)blocks);
   return dim3(1u << 20, (unsigned)((blocks + (1 << 20) - 1) >> 20));
 }
-__device__ inline long long block_number() { return blockIdx.x + (long long)blockIdx.y * gridDim.x; }
+__device__ inline long long block_number() { return blockIdx.x + ((long long)blockIdx.y << 20); }
 
 inline bool dtype_ok(int dtype) { return dtype >= K3_F32 && dtype <= K3_BF16; }
 inline size_t dtype_size(int dtype) { return dtype == K3_F32 ? 4 : 2; }

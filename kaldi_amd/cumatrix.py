@@ -13,6 +13,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 
 _current_device = torch.cuda.current_device
 _F32, _I32 = torch.float32, torch.int32
+_MOST = 0x7fffffff      # the C entries' sizes are int32, and ctypes would cut what is larger
 _devices = [torch.device("cuda", i) for i in range(64)]
 
 def _refuse(what): raise _l.K3Error(what)
@@ -21,10 +22,11 @@ def _rows(m, name):
     t = m.t if type(m) is CuMatrix else m
     try: dt = _DTYPES[t.dtype]; r, c = t.shape; s0, s1 = t.stride(); i = t.get_device()
     except (AttributeError, KeyError, ValueError, RuntimeError): _refuse(f"{name}: a matrix of float32, float16 or bfloat16 is wanted")
-    if r > 0x7fffffff or c > 0x7fffffff: _refuse(f"{name}: {r} x {c}: at most 2^31 - 1 rows and columns")      # (the C entries' sizes are int32, and ctypes would cut them)
+    if not 1 < r <= _MOST: s0 = c if r <= 1 else -1
+    if (s1 != 1 and c > 1) or not s0 >= c <= _MOST:
+        if r > _MOST or c > _MOST: _refuse(f"{name}: {r} x {c}: at most 2^31 - 1 rows and columns")
+        _refuse(f"{name}: rows must be contiguous and must not overlap (strides {s0}, {s1})")
     if i < 0: _refuse(f"{name}: not on a GPU")
-    if r <= 1: s0 = c
-    if (s1 != 1 and c > 1) or s0 < c: _refuse(f"{name}: rows must be contiguous and must not overlap (strides {s0}, {s1})")
     return dt, t.data_ptr(), s0, r, c, i
 def _like_rows(m, x, name):
     """a second matrix of x's shape, type and device (x: what _rows gave): (pointer, leading dimension)"""
