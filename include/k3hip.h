@@ -601,7 +601,7 @@ int k3_label_logprobs(int32_t dtype, const void *d_z, int64_t ld, const int32_t 
                       float *d_alt_log_probs, int32_t *d_alt_labels, void *d_workspace, int64_t workspace_bytes, int32_t rows, int32_t cols, void *stream);
 /* The derivative of sum_r d_log_prob_deriv[r] log q_y(r) + d_entropy_deriv[r] entropy(r) with respect to z, into d_dz (overwritten; may be z).  d_stats (and d_entropy, where
  * d_entropy_deriv is given) are the forward pass's; either derivative may be null (0); a row without a label has no first term; a row of
- * nothing but -inf gets zeros, and so does one whose two derivatives are 0, whatever it holds. */
+ * nothing but -inf gets zeros, and so does one whose two derivatives are 0, whatever it holds.  At most 2^31 - 4096 columns. */
 int k3_label_logprobs_deriv(int32_t dtype, const void *d_z, int64_t ld, const int32_t *d_labels, const float *d_stats, const float *d_entropy, const float *d_log_prob_deriv,
                             const float *d_entropy_deriv, void *d_dz, int64_t ldd, int32_t rows, int32_t cols, void *stream);
 /* Distillation from a teacher's top logits: row r has num_entries (1 .. 1024) pairs of a teacher value (of z's type) and its column; a column outside 0 .. cols - 1, -1 for instance =

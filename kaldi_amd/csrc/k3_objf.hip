@@ -632,6 +632,7 @@ template <typename T> int distill(DistillArgs p, void *workspace, hipStream_t st
 }
 
 const int kMaxCols = kMaxSplits * 4 * 64 * 8 * 4;      // 64 parts of what a workgroup of four wavefronts holds of float32 columns: 2^19
+const int kMaxDerivCols = 0x7fffffff - 4095;                // column numbers of k3_label_deriv_kernel's threads that run ahead of a row's end still fit 32 bits
 
 }  // namespace
 
@@ -668,6 +669,7 @@ extern "C" int k3_label_logprobs_deriv(int32_t dtype, const void *d_z, int64_t l
                                        const float *d_entropy_deriv, void *d_dz, int64_t ldd, int32_t rows, int32_t cols, void *stream) {
   K3_REQUIRE(dtype_ok(dtype), "k3_label_logprobs_deriv: unknown type");
   K3_REQUIRE(rows >= 0 && cols >= 1 && ld >= cols && ldd >= cols, "k3_label_logprobs_deriv: bad argument");
+  if (cols > kMaxDerivCols) { set_error("k3_label_logprobs_deriv: at most %d columns", kMaxDerivCols); return K3_ERR_UNSUPPORTED; }
   if (rows == 0) return K3_OK;
   K3_REQUIRE(d_z && d_dz && d_stats && (d_labels || !d_log_prob_deriv) && (d_entropy || !d_entropy_deriv), "k3_label_logprobs_deriv: null input");
   const Span z = matrix_span(d_z, ld, rows, cols, dtype_size(dtype)), dz = matrix_span(d_dz, ldd, rows, cols, dtype_size(dtype));

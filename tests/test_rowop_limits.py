@@ -21,3 +21,10 @@ def test_sizes_that_do_not_fit_32_bits():
         for call in (lambda: cm.LayerNormPerRow(t, None, None, 1e-5, t), lambda: cm.AffinePerRow(t, t, None, "none", None, t), lambda: cm.DiffAffinePerRow(t, t, None, "none", t), lambda: ob.LabelLogProbs(t, None),
                      lambda: cm.DiffLayerNormPerRow(t, t, None, None, None), lambda: ob.DiffLabelLogProbs(t, None, None, None, None, None, t), lambda: ob.ComputeDistillObjfAndDeriv(ob.DistillationOptions(), t, t, t, None, None)):
             with pytest.raises(K3Error, match="2\\^31"): call()
+
+def test_label_derivative_of_rows_whose_column_numbers_pass_32_bits():
+    L = _l.load(); most = (1 << 31) - 4096; wide = 1 << 32
+    for dtype in (0, 1, 2):
+        f = lambda cols: L.k3_label_logprobs_deriv(dtype, P, wide, None, P, None, None, None, P, wide, 0, cols, None)  # noqa: E731
+        for cols in (most + 1, (1 << 31) - 2048, (1 << 31) - 1): refused(f(cols), "at most")
+        assert f(most) == 0      # (without rows: nothing is queued)
