@@ -567,7 +567,8 @@ int k3_chain_objf_and_deriv(k3_chain_den *den, k3_chain_supervision *sup, const 
 typedef enum { K3_F32 = 0, K3_F16 = 1, K3_BF16 = 2 } k3_dtype;
 /* Layer norm of every row: y = (x - mean) inv_std scale + offset with inv_std = 1 / sqrt(var + eps), var = the mean square of x - mean.  Stands beside cu::NormalizePerRow
  * (cudamatrix/cu-math.h:272), which takes no mean away.  d_scale / d_offset [cols] may be null (1 / 0); d_mean / d_inv_std [rows] (null: not kept) are what the backward pass takes.
- * y may be x.  cols = 0 or rows = 0: nothing to do.  At most 2^31 - 1024 columns. */
+ * y may be x.  cols = 0 or rows = 0: nothing to do.  At most 2^31 - 1024 columns.  A row that holds an infinity or a NaN has inv_std NaN and is NaN throughout; one whose differences from
+ * the mean pass the root of float32's range (1.8e19) has inv_std 0. */
 int k3_layer_norm_forward(int32_t dtype, const void *d_x, int64_t ldx, const float *d_scale, const float *d_offset, float eps, void *d_y, int64_t ldy,
                           float *d_mean, float *d_inv_std, int32_t rows, int32_t cols, void *stream);
 /* Its derivatives from dy: d_dx (null: not wanted; may be dy or x), d_dscale / d_doffset [cols] (null: not wanted), overwritten, or added to with accumulate != 0 (rows = 0 then leaves
@@ -579,14 +580,16 @@ int k3_layer_norm_backward(int32_t dtype, const void *d_x, int64_t ldx, const vo
                            int32_t rows, int32_t cols, void *stream);
 /* An affine layer in half precision (dtype K3_F16 or K3_BF16): pre = x W^T + bias, y = act(pre) + residual, x [rows x inner], W [cols x inner] (AffineComponent's linear_params),
  * d_bias float32 [cols] (null: 0), d_residual [rows x cols] (null: none; y may be it).  d_pre (null: not kept) receives pre as the backward pass takes it.  Products are summed in float32 and
- * a result is rounded once.  Stands beside k3_mat_add_mat_mat, which is float32 and has no epilogue.  Workspace (16-byte aligned): k3_affine_forward_workspace. */
+ * a result is rounded once.  Stands beside k3_mat_add_mat_mat, which is float32 and has no epilogue.  At most 2^30 rows, 2^20 inner and 2^22 cols, with rows (inner + cols) < 2^42.  Workspace (16-byte aligned):
+ * k3_affine_forward_workspace. */
 typedef enum { K3_ACT_NONE = 0, K3_ACT_RELU = 1, K3_ACT_SIGMOID = 2, K3_ACT_TANH = 3, K3_ACT_SWISH = 4 /* z sigmoid(z) */, K3_ACT_GELU = 5 /* z (1 + erf(z / sqrt 2)) / 2 */ } k3_activation;
 int64_t k3_affine_forward_workspace(int32_t rows, int32_t inner, int32_t cols);
 int k3_affine_forward(int32_t dtype, int32_t act, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const float *d_bias, const void *d_residual, int64_t ldr, void *d_y,
                       int64_t ldy, void *d_pre, int64_t ldp, void *d_workspace, int64_t workspace_bytes, int32_t rows, int32_t inner, int32_t cols, void *stream);
 /* Its derivatives from dy: dz = dy act'(pre) (d_pre not read for K3_ACT_NONE), d_dx = dz W and d_dw = dz^T x (of the matrices' type), d_db [cols] = the sum of dz over the rows (float32);
  * each may be null (not wanted), and what is given is overwritten.  (The residual's derivative is dy itself.)  Where there is an activation, dz is rounded to the matrices' type for the two
- * products, not for d_db.  Sums are taken in a fixed order.  rows = 0 clears d_dw and d_db.  Workspace (16-byte aligned): k3_affine_backward_workspace. */
+ * products (in float16 what is below 2^-25 is lost: dy is to be scaled up, as usual there), not for d_db.  Sums are taken in a fixed order.  rows = 0 clears d_dw and d_db.  Sizes as
+ * above.  Workspace (16-byte aligned): k3_affine_backward_workspace. */
 int64_t k3_affine_backward_workspace(int32_t act, int32_t rows, int32_t inner, int32_t cols);
 int k3_affine_backward(int32_t dtype, int32_t act, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_pre, int64_t ldp, const void *d_dy, int64_t lddy,
                        void *d_dx, int64_t lddx, void *d_dw, int64_t lddw, float *d_db, void *d_workspace, int64_t workspace_bytes, int32_t rows, int32_t inner, int32_t cols, void *stream);
@@ -605,7 +608,7 @@ int k3_label_logprobs(int32_t dtype, const void *d_z, int64_t ld, const int32_t 
 int k3_label_logprobs_deriv(int32_t dtype, const void *d_z, int64_t ld, const int32_t *d_labels, const float *d_stats, const float *d_entropy, const float *d_log_prob_deriv,
                             const float *d_entropy_deriv, void *d_dz, int64_t ldd, int32_t rows, int32_t cols, void *stream);
 /* Distillation from a teacher's top logits: row r has num_entries (1 .. 1024) pairs of a teacher value (of z's type) and its column; a column outside 0 .. cols - 1, -1 for instance =
- * not used.  With p = softmax(values / T) over the used entries, q = softmax(z / T) over all columns and T = temperature:
+ * not used.  With p = softmax(values / T) over the used entries, q = softmax(z / T) over all columns and T = temperature (1e-3 .. 1e3):
  *   d_objf[r] = w_r T^2 sum_k p_k (log q_{i_k} - log p_k)      (the negative divergence of p from q: to be maximised, as the chain objective is)
  *   d_dz[r][j] = w_r T (sum of p_k over i_k = j  -  q_j)       (its derivative; overwritten, may be z; d_dz null: not wanted)
  * A column may come more than once.  d_weights [rows] (null: 1).  A row without a used entry (or with nothing but -inf in them), or of weight 0, has objective 0 and zeros, whatever z

@@ -4,8 +4,9 @@
 // All three products are C[m][n] = sum_k A(m, k) B(n, k) on the matrix cores (16 x 16 x 32, float32 accumulation); an operand's contraction index is its contiguous one (x, W, dz for dx) or
 // its row index (W for dx; dz and x for dW).  The former is read from LDS as it lies (16 bytes of one row per lane), the latter with the transposing LDS read (4 contraction steps of
 // 16 rows per 16 lanes), so no operand is ever transposed in memory.
-// Measured in bfloat16: 8192 x 8192 x 8192 948 us forward (1.16 PFLOP/s), 1028 dx, 934 dW; 42752 x 1536 x 1536 with ReLU, bypass and the activation's input kept 236 us (198 without them: the
-// epilogues of all compute units come at the same time); 25600 x 768 x 6024 292 us dx, 290 dW (matrix cores busy 35 % of the chip's cycles by counters; its rows of 12048 bytes straddle cache lines).
+// Measured in bfloat16: 8192 x 8192 x 8192 958 us forward (1.15 PFLOP/s), 1042 dx, 950 dW; 42752 x 1536 x 1536 with ReLU, bypass and the activation's input kept 236 us (191 without them: the
+// epilogues of all compute units come at the same time); 25600 x 768 x 6024 287 us dx, 282 dW (matrix cores busy 35 % of the chip's cycles by counters: what their loads wait for stands at
+// k3_affine_product_kernel).
 #include "k3_rowops.h"
 #include <algorithm>
 #include <type_traits>
@@ -446,7 +447,9 @@ template <typename T> __device__ inline void slopes(int act, Packed z, float (&d
     default: return;
   }
 }
-// dz = dy act'(pre), rounded to the matrices' type for the products (null: dz is dy), and the sums over a strip of rows of the unrounded values: sums [strip][cols]; a workgroup takes 64
+// dz = dy act'(pre), rounded to the matrices' type for the products (null: dz is dy), and the sums over a strip of rows of the unrounded values: sums [strip][cols].  The rounding is what
+// the matrix cores ask for: float32's other bits would go into a second half and a second product each.  It is as large as that of dy itself (none for ReLU): dx and dW of 4096 x 768 <- 1536
+// with gelu are 2.3e-3 off in bfloat16 where one rounding makes 1.7e-3 (2.9e-4 and 2.1e-4 in float16, in which a dz below 2^-25 is lost).  A workgroup takes 64
 // chunks of 8 columns by one strip, each of its 4 wavefronts every 4th row, the next one on its way while this one is worked on.  (Small code counts: short calls are over before much of it has
 // been fetched.  4 rows at a time, with their activations written out, took 12.8 us on 208 rows of 173 columns.)
 template <typename T> __global__ __launch_bounds__(256) void k3_affine_slope_kernel(int act, const T *dy, long long lddy, const T *pre, long long ldp, T *dz, long long lddz, float *sums,

@@ -194,7 +194,8 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
   }
 }
 
-// one workgroup per row, any width: the row is read once for each of the sums and once more for the result
+// one workgroup per row, any width: the row is read once for each of the sums and once more for the result, element by element (float32 2000 x 20011 123 us forward, 153 backward, bfloat16
+// 86 and 113: 2.6 and 1.9 TB/s of what has to be moved forward)
 template <typename T> __global__ __launch_bounds__(256) void k3_ln_forward_loop_kernel(const T *x, long long ldx, const float *scale, const float *offset, float eps,
                                                                                        T *y, long long ldy, float *mean, float *inv_std, int cols) {
   __shared__ float sh[12];
@@ -283,7 +284,7 @@ const int kMaxCols = 0x7fffffff - 1023;      // column numbers of threads that r
 const int kMaxParamCols = (1 << 28) - 64;    // k3_ln_param_join_kernel has 16 threads per column, and a launch less than 2^32
 
 // wavefronts per row and chunks per thread: the fewest wavefronts that hold the row with at most 16 (float) or 24 elements per thread, and no more than 16 of them (then 12 or 16
-// elements: a workgroup of 1024 has 128 registers per thread, and one chunk more spills in the backward pass); {0, 0} = too wide
+// elements: a workgroup of 1024 has 128 registers per thread, of which the backward pass already spills 4 with 12 floats and 34 with 16 halves); {0, 0} = too wide
 struct Shape { int nw, e; };
 template <typename T> Shape shape_of(int cols) {
   const int chunks = (cols + Chunk<T>::N - 1) / Chunk<T>::N, most = sizeof(T) == 4 ? 4 : 3;

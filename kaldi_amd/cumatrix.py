@@ -7,7 +7,7 @@ from . import lib as _l
 def _st(): return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 # ---- arguments of the operators that take matrices of any k3_dtype: CuMatrix objects or 2-dimensional tensors whose rows are contiguous, all on one device (which need not be
-# the current one); the kernels run on that device's current stream
+# the current one); the kernels run on that device's current stream.  What a call writes shares no element with its other operands, unless it may be one of them (K3Error otherwise)
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # k3_dtype
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
 
