@@ -54,3 +54,16 @@ def test_distillation_with_entries_at_masked_columns(cols, dtype):
         assert_within(f, want, e * mag, "objf"); assert_within(alone, want, e * mag, "objf alone")
         P = torch.zeros_like(lq).scatter_add_(1, at, p); d = w.double()[:, None] * T * (P - lq.exp()); off = e * w.double().abs()[:, None] * T * (P + lq.exp())
         assert_within(dz, d, half_step(dtype) * (d.abs() + off) + off + tiny(dtype), "dz")
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [67, 489, 9001, 20794, 140001])
+def test_distillation_with_all_entries_at_masked_columns(cols, dtype):
+    """the probabilities add up to 1 but for their roundings, and the objective to w T (lowest - M): finite, as the bounds above have it, where w T is below 1"""
+    from kaldi_amd.objective import ComputeDistillObjfAndDeriv, DistillationOptions
+    g = generator(cols); n, N, c = 64, 40, cols // 2; z = torch.randn(n, cols, generator=g, device="cuda").to(dtype); z[:, c:] = torch.finfo(dtype).min; idx = torch.randint(c, cols, (n, N), generator=g, device="cuda").to(torch.int32)
+    t = torch.randn(n, N, generator=g, device="cuda").to(dtype); w = (0.1 + 0.3 * torch.rand(n, generator=g, device="cuda")); f, dz, alone = torch.empty(n, device="cuda"), empty_like(z), torch.empty(n, device="cuda")
+    for T in (0.5, 1.0, 2.0):
+        o = DistillationOptions(T); ComputeDistillObjfAndDeriv(o, z, t, idx, w, f, dz); ComputeDistillObjfAndDeriv(o, z, t, idx, w, alone); D = 40.0 + 8.0 / T; e = S(cols, D) + S(64, D)
+        lp = torch.log_softmax(t.double() / T, 1); x = (z.double() - z.double().amax(1, keepdim=True)) / T; lq = x - torch.logsumexp(x, 1, keepdim=True); p = lp.exp(); lqk = lq.gather(1, idx.long())
+        want = w.double() * T * T * (p * (lqk - lp)).sum(1); off = e * w.double() * T * T * (p * (lqk.abs() + lp.abs() + 1)).sum(1); assert (want.abs() < 2.8e38).all(); assert_within(f, want, off, "objf"); assert_within(alone, want, off, "objf alone")
+        P = torch.zeros_like(lq).scatter_add_(1, idx.long(), p); d = w.double()[:, None] * T * (P - lq.exp()); off = e * w.double()[:, None] * T * (P + lq.exp()); assert_within(dz, d, half_step(dtype) * (d.abs() + off) + off + tiny(dtype), "dz")
