@@ -401,16 +401,19 @@ template <typename T, int NW> __device__ inline Teacher teacher_softmax(const Di
   }
   return Teacher{block_sum<NW>(s, sh + NW), m != -kInf && !(p.weights && p.weights[row] == 0.0f)};
 }
-// T / 4 sum_k p_k (log q_k - log p_k) from the student's M and s; in every thread.  Differences stay in the logits' units and are divided by the teacher's sum (at least 1) one by one: in
-// those of the exponentials, or summed before the division, one with a lowest value in it would overflow, which the objective does not.  (A quarter: where all entries have it, the sum is the
-// lowest value itself, give or take its roundings.)
-template <int NW> __device__ inline float teacher_objf(const DistillArgs &p, const Entry *entry, Teacher w, float m, float s, int t, float *sh) {
+// sum_k e_k ((z_k - M) - (v_k - max v)) / 4096, in every thread.  The differences stay in the logits' units, and 1024 of them are added up well within float32's range: in the units of the
+// exponentials, or as they are, those that have a lowest value in them would overflow, which the objective does not
+constexpr float kShrink = 1.0f / (4 * kMaxTeacher);
+template <int NW> __device__ inline float teacher_differences(const DistillArgs &p, const Entry *entry, float m, int t, float *sh) {
   float f = 0.0f;
-  const float r = 0.25f / w.sum;
   for (int k = t; k < p.top; k += 64 * NW)
-    if (!(entry[k].e == 0.0f)) f += entry[k].e * (r * (entry[k].z - m - entry[k].d));
-  f = block_sum<NW>(f, sh);
-  return m == -kInf && s == s ? -kInf : f + 0.25f * p.temperature * kLn2 * (log2f(w.sum) - log2f(s));
+    if (!(entry[k].e == 0.0f)) f += entry[k].e * (kShrink * (entry[k].z - m - entry[k].d));
+  return block_sum<NW>(f, sh);
+}
+// w T^2 sum_k p_k (log q_k - log p_k) from them and the student's M and s, with wt = w T; by one thread
+__device__ inline float teacher_objf(const DistillArgs &p, Teacher w, float wt, float m, float s, float f) {
+  if (!w.live) return 0.0f;
+  return m == -kInf && s == s ? wt * -kInf : wt / kShrink * (f / w.sum + kShrink * p.temperature * kLn2 * (log2f(w.sum) - log2f(s)));
 }
 
 // One row per NW wavefronts, held in registers from the sums to the derivative: read once, written once.  The teacher's columns are corrected behind the row's own store (by the same
@@ -446,8 +449,8 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
   const bool empty = s == 0.0f;      // (the row's largest value adds 1: nothing but -inf)
   if (empty) m = -kInf;
   const float w = (p.weights ? p.weights[row] : 1.0f) * p.temperature;
-  const float f = teacher_objf<NW>(p, entry, teacher, m, s, t, sh + 4 * NW);
-  if (t == 0) p.objf[row] = teacher.live ? 4.0f * w * f : 0.0f;
+  const float f = teacher_differences<NW>(p, entry, m, t, sh + 4 * NW);
+  if (t == 0) p.objf[row] = teacher_objf(p, teacher, w, m, s, f);
   if (!p.dz) return;
   T *dz = (T *)p.dz + row * p.ldd;
   if (!teacher.live || empty) {
@@ -477,9 +480,9 @@ template <typename T> __global__ __launch_bounds__(64) void k3_distill_join_kern
   const Teacher teacher = teacher_softmax<T, 1>(p, row, entries, teacher_max, t, nullptr);
   float m, s, u;
   join_parts(p.partial + row * p.splits, p.splits, p.a, m, s, u);
-  const float w = (p.weights ? p.weights[row] : 1.0f) * p.temperature, f = teacher_objf<1>(p, entries, teacher, m, s, t, nullptr);
+  const float w = (p.weights ? p.weights[row] : 1.0f) * p.temperature, f = teacher_differences<1>(p, entries, m, t, nullptr);
   if (t == 0) {
-    p.objf[row] = teacher.live ? 4.0f * w * f : 0.0f;
+    p.objf[row] = teacher_objf(p, teacher, w, m, s, f);
     if (p.dz) p.coef[row] = make_float4(m, -w / s, w, teacher.live && !(m == -kInf && s == s) ? 1.0f : 0.0f);
   }
   if (p.dz)
