@@ -4,8 +4,8 @@
 // All three products are C[m][n] = sum_k A(m, k) B(n, k) on the matrix cores (16 x 16 x 32, float32 accumulation); an operand's contraction index is its contiguous one (x, W, dz for dx) or
 // its row index (W for dx; dz and x for dW).  The former is read from LDS as it lies (16 bytes of one row per lane), the latter with the transposing LDS read (4 contraction steps of
 // 16 rows per 16 lanes), so no operand is ever transposed in memory.
-// Measured in bfloat16: 8192 x 8192 x 8192 958 us forward (1.15 PFLOP/s), 1042 dx, 950 dW; 42752 x 1536 x 1536 with ReLU, bypass and the activation's input kept 236 us (191 without them: the
-// epilogues of all compute units come at the same time); 25600 x 768 x 6024 287 us dx, 282 dW (matrix cores busy 35 % of the chip's cycles by counters: what their loads wait for stands at
+// Measured in bfloat16: 8192 x 8192 x 8192 938 us forward (1.17 PFLOP/s), 1036 dx, 941 dW; 42752 x 1536 x 1536 with ReLU, bypass and the activation's input kept 234 us (187 without them: the
+// epilogues of all compute units come at the same time); 25600 x 768 x 6024 286 us dx, 280 dW (matrix cores busy 36 % of the chip's cycles by counters: what their loads wait for stands at
 // k3_affine_product_kernel).
 #include "k3_rowops.h"
 #include <algorithm>

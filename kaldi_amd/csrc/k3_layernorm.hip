@@ -194,7 +194,7 @@ template <typename T, int NW, int E> __global__ __launch_bounds__(NW == 1 ? 256 
   }
 }
 
-// one workgroup per row, any width: the row is read once for each of the sums and once more for the result, element by element (float32 2000 x 20011 123 us forward, 153 backward, bfloat16
+// one workgroup per row, any width: the row is read once for each of the sums and once more for the result, element by element (float32 2000 x 20011 123 us forward, 154 backward, bfloat16
 // 86 and 113: 2.6 and 1.9 TB/s of what has to be moved forward)
 template <typename T> __global__ __launch_bounds__(256) void k3_ln_forward_loop_kernel(const T *x, long long ldx, const float *scale, const float *offset, float eps,
                                                                                        T *y, long long ldy, float *mean, float *inv_std, int cols) {

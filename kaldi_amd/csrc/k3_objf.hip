@@ -4,9 +4,9 @@
 //   distillation, p = softmax of a row's teacher values:  objf = w T^2 sum_k p_k (log q_{i_k} - log p_k),  d objf / d z_j = w T (sum of p_k over i_k = j  -  q_j)
 // Elements are held as they are stored and widened where they are used; statistics, sums and exponentials are float32.  The difference is taken before the product: a z_j alone would
 // overflow at the lowest values of float32 and bfloat16, which masks are made of.
-// Bound by memory, a row being read once (and its derivative written once): scores of float32 42752 x 6024 with 4 alternatives 166 us (6.2 TB/s), label derivative of bfloat16 2000 x 50001
-// 78 us (5.1), distillation with derivative of float32 6400 x 6024 66 us (4.6) and of bfloat16 4096 x 128000 512 us (4.1: a row fills a compute unit's registers, and its
-// vector instructions, 53 to 55 % of its cycles by counters, run under its own loads and stores only in part).
+// Bound by memory, a row being read once (and its derivative written once): scores of float32 42752 x 6024 with 4 alternatives 165 us (6.2 TB/s), label derivative of bfloat16 2000 x 50001
+// 78 us (5.1), distillation with derivative of float32 6400 x 6024 66 us (4.6) and of bfloat16 4096 x 128000 509 us (4.1: a row fills a compute unit's registers, and its
+// vector instructions, 55 % of its cycles by counters, run under its own loads and stores only in part).
 #include "k3_rowops.h"
 #include <algorithm>
 #include <type_traits>
@@ -75,7 +75,7 @@ template <int NW> struct TopShared { unsigned long long cand[kCandidates + 8]; u
 // column(e): its column alone; lane_max: the thread's largest value (-inf: none).
 // Every lane's largest element bounds what can be among the best: with t = the top-th largest of the lanes' maxima, `top` elements are >= t, so only elements >= t (as a rule a few more
 // than `top`) are gathered and ranked by counting.  Where more than fit are >= t (many equal values), the best are taken one after another instead,
-// each with a read of the row (float32 42752 x 6024 of one value, 4 alternatives: 1212 us where random ones take 193).
+// each with a read of the row (float32 42752 x 6024 of one value, 4 alternatives: 1215 us where random ones take 192).
 template <int NW, int E, int N, typename V, typename P, typename C, typename G, typename F>
 __device__ inline void emit_top(V value, P pick, C column, G fetch, float lane_max, int top, TopShared<NW> &sh, F emit) {
   constexpr int TPR = 64 * NW;
